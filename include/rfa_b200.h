@@ -232,6 +232,53 @@ int rfa_bwd_local(const void* q, const void* k, const void* v, const void* out, 
                   void* stream);
 
 /*
+ * Attention with modified scores.  For query i and key j (positions in the whole sequence)
+ *   x = softmax_scale * q_i . k_j;  y = softcap > 0 ? softcap * tanh(x / softcap) : x;  z = y - slope[h] * |i - j|
+ * and the softmax of a row runs over the keys it sees: all of them, those up to its own position (causal), or those that a
+ * mask buffer names.  A row that sees no key gets out = 0 and lse = -inf, and takes no part in any gradient.
+ */
+typedef struct rfa_score_args {
+  float softmax_scale;      /* > 0 */
+  float softcap;            /* > 0: cap of the scores; 0: none */
+  const float* slopes;      /* NULL, or distance slopes (>= 0 or < 0): [Hq], or [B, Hq] with slopes_per_batch */
+  int slopes_per_batch;
+  int causal;               /* without a mask: key j is seen by query i when j <= i; with one: as the mask was built */
+  const int* mask;          /* NULL, or what rfa_document_mask wrote, 16-byte aligned */
+  int shards, q_shard, k_shard; /* the sequence is `shards` blocks of S rows; queries are block q_shard, keys block k_shard */
+} rfa_score_args;
+
+/* int32 elements of a mask buffer for B rows of shards * S tokens; 0 when the sizes are not supported. */
+size_t rfa_mask_elems(int B, int S, int shards);
+
+/*
+ * Document mask.  Batch row b (row 0 for all when cu_rows is 1) consists of the documents [cu[d], cu[d+1]), d < n_docs, of
+ * cu [cu_rows, n_docs + 1] (int32, device memory, not decreasing); tokens of different documents do not see each other,
+ * tokens before cu[0] or from cu[n_docs] on are padding.  With `causal` a key is seen by the queries of its document that
+ * do not precede it, and, where prefix [cu_rows, n_docs] is given, the first prefix[d] tokens of document d by all of them.
+ * Positions outside the sequence count as its ends.  Two launches; no host synchronisation.
+ */
+int rfa_document_mask(const int* cu, const int* prefix, int cu_rows, int n_docs, int B, int S, int shards, int causal,
+                      int* mask, void* stream);
+
+/*
+ * rfa_fwd_hop, rfa_bwd_hop and rfa_bwd_local with modified scores, for blocks of equal length S (q, k, v of [B,S,H,D]).
+ * State, scratch and results as there; rfa_bwd_prepare and rfa_bwd_dq_finalize serve both.  `args` is host memory, read
+ * before the call returns.  Padding rows of q, k, v and dout may hold anything; their out and gradients are zero.
+ *  dq_order  NULL, or rfa_dq_order_elems(B,S,Hq,D) counters: bit-reproducible gradients (every tile that the causal rule
+ *            alone would visit is visited then, whatever the mask leaves of it)
+ */
+int rfa_scored_fwd_hop(const void* q, const void* k, const void* v, float* acc, float* m, float* l, void* out, float* lse,
+                       int B, int S, int Hq, int Hkv, int D, int dtype, const rfa_score_args* args, int first, int last,
+                       int* status, void* stream);
+int rfa_scored_bwd_hop(const void* q, const void* k, const void* v, const void* dout, const float* lse2,
+                       const float* delta, float* dq_acc, float* dkdv_out, int B, int S, int Hq, int Hkv, int D, int dtype,
+                       const rfa_score_args* args, int* dq_order, int* status, void* stream);
+int rfa_scored_bwd_local(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
+                         float* delta, float* lse2, float* dq_acc, float* dkdv, void* dq, void* dk, void* dv, int B, int S,
+                         int Hq, int Hkv, int D, int dtype, const rfa_score_args* args, int* dq_order, int* status,
+                         void* stream);
+
+/*
  * Packs K and V ([B, Skv, Hkv, D] each, `bytes_each` bytes) into one contiguous
  * [2, B, Skv, Hkv, D] transport buffer.  Replaces `kv_send[0].copy_(k);
  * kv_send[1].copy_(v)` (optimized_ring_flash_attn.py:836-838, 974-976).

@@ -6,6 +6,7 @@ from .compat import (  # noqa: F401
     ring_flash_attn_qkvpacked_func,
 )
 from .schedule import shutdown  # noqa: F401
+from .scored import DocumentMask, document_mask, scored_flash_attn, scored_flash_attn_with_lse  # noqa: F401
 
 __all__ = [
     "ring_flash_attn",
@@ -13,6 +14,10 @@ __all__ = [
     "ring_flash_attn_func",
     "ring_flash_attn_kvpacked_func",
     "ring_flash_attn_qkvpacked_func",
+    "scored_flash_attn",
+    "scored_flash_attn_with_lse",
+    "document_mask",
+    "DocumentMask",
     "deterministic",
     "balanced",
     "check",

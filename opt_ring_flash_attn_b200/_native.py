@@ -48,6 +48,11 @@ SIGNATURES = {
     "rfa_dq_order_elems": (_sz, [_i, _i, _i, _i]),
     "rfa_bwd_hop_ordered": (_i, [_vp] * 9 + [_i] * 7 + [_f] + [_i] * 4 + [_vp, _vp, _vp]),
     "rfa_bwd_local": (_i, [_vp] * 13 + [_i] * 6 + [_f, _i, _vp, _vp, _vp]),
+    "rfa_mask_elems": (_sz, [_i] * 3),
+    "rfa_document_mask": (_i, [_vp] * 2 + [_i] * 6 + [_vp] * 2),
+    "rfa_scored_fwd_hop": (_i, [_vp] * 8 + [_i] * 6 + [_vp] + [_i] * 2 + [_vp] * 2),
+    "rfa_scored_bwd_hop": (_i, [_vp] * 8 + [_i] * 6 + [_vp] * 4),
+    "rfa_scored_bwd_local": (_i, [_vp] * 13 + [_i] * 6 + [_vp] * 4),
     "rfa_noalloc_scratch_bytes": (_sz, []),
     "rfa_bwd_hop_noalloc": (_i, [_vp] * 9 + [_i] * 7 + [_f] + [_i] * 2 + [_vp, _vp]),
     "rfa_dkdv_accumulate": (_i, [_vp, _vp, _vp, _sz, _vp]),
@@ -222,6 +227,70 @@ def bwd_local(q, k, v, out, dout, lse, delta, lse2, dq_acc, dkdv, dq, dk, dv, so
             B, S, Hq, k.shape[2], D, DTYPE_CODES[q.dtype], float(softmax_scale), int(causal), _ptr(dq_order),
             status.data_ptr(), _stream(stream, q))
     _check(rc, "rfa_bwd_local", kernels=3)
+
+
+class ScoreArgs(ctypes.Structure):
+    """``rfa_score_args`` of the C header."""
+    _fields_ = [("softmax_scale", _f), ("softcap", _f), ("slopes", _vp), ("slopes_per_batch", _i), ("causal", _i),
+                ("mask", _vp), ("shards", _i), ("q_shard", _i), ("k_shard", _i)]
+
+
+def score_args(softmax_scale: float, softcap: float, slopes: Optional[torch.Tensor], causal: bool,
+               mask: Optional[torch.Tensor], shards: int = 1, q_shard: int = 0, k_shard: int = 0) -> ScoreArgs:
+    return ScoreArgs(softmax_scale, softcap, _ptr(slopes), int(slopes is not None and slopes.dim() == 2), int(causal),
+                     _ptr(mask), shards, q_shard, k_shard)
+
+
+def mask_elems(B: int, S: int, shards: int) -> int:
+    n = load().rfa_mask_elems(B, S, shards)
+    if n == 0:
+        raise RuntimeError(f"unsupported sizes for a document mask: B={B} S={S} shards={shards}")
+    return n
+
+
+def document_mask(cu: torch.Tensor, prefix: Optional[torch.Tensor], B: int, S: int, shards: int, causal: bool,
+                  mask: torch.Tensor, stream=None) -> None:
+    """``cu`` int32 ``[n + 1]`` or ``[B, n + 1]``, ``prefix`` int32 ``[n]`` or ``[B, n]``, into the buffer ``mask``."""
+    rows = 1 if cu.dim() == 1 else cu.shape[0]
+    with _on_device(mask):
+        rc = load().rfa_document_mask(_ptr(cu), _ptr(prefix), rows, cu.shape[-1] - 1, B, S, shards, int(causal), _ptr(mask),
+                                      _stream(stream, mask))
+    _check(rc, "rfa_document_mask", kernels=2)
+
+
+def scored_fwd_hop(q, k, v, acc, m, l, out, lse, args: ScoreArgs, first: bool, last: bool, status, stream=None) -> None:
+    """:func:`fwd_hop` with modified scores (``rfa_scored_fwd_hop``)."""
+    B, S, Hq, D = q.shape
+    with _on_device(q):
+        rc = load().rfa_scored_fwd_hop(_ptr(q), _ptr(k), _ptr(v), _ptr(acc), _ptr(m), _ptr(l), _ptr(out), _ptr(lse),
+                                       B, S, Hq, k.shape[2], D, DTYPE_CODES[q.dtype], ctypes.byref(args), int(first),
+                                       int(last), _ptr(status), _stream(stream, q))
+    _check(rc, "rfa_scored_fwd_hop")
+
+
+def scored_bwd_hop(q, k, v, dout, lse2, delta, dq_acc, dkdv_out, args: ScoreArgs, status, stream=None,
+                   dq_order: Optional[torch.Tensor] = None) -> None:
+    """:func:`bwd_hop` with modified scores (``rfa_scored_bwd_hop``)."""
+    B, S, Hq, D = q.shape
+    assert dq_order is None or (dq_order.dtype == torch.int32 and dq_order.numel() >= dq_order_elems(B, S, Hq, D))
+    with _on_device(q):
+        rc = load().rfa_scored_bwd_hop(_ptr(q), _ptr(k), _ptr(v), _ptr(dout), _ptr(lse2), _ptr(delta), _ptr(dq_acc),
+                                       _ptr(dkdv_out), B, S, Hq, k.shape[2], D, DTYPE_CODES[q.dtype], ctypes.byref(args),
+                                       _ptr(dq_order), _ptr(status), _stream(stream, q))
+    _check(rc, "rfa_scored_bwd_hop")
+
+
+def scored_bwd_local(q, k, v, out, dout, lse, delta, lse2, dq_acc, dkdv, dq, dk, dv, args: ScoreArgs, status, stream=None,
+                     dq_order: Optional[torch.Tensor] = None) -> None:
+    """:func:`bwd_local` with modified scores (``rfa_scored_bwd_local``)."""
+    B, S, Hq, D = q.shape
+    assert dq_order is None or (dq_order.dtype == torch.int32 and dq_order.numel() >= dq_order_elems(B, S, Hq, D))
+    with _on_device(q):
+        rc = load().rfa_scored_bwd_local(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(dout), _ptr(lse), _ptr(delta), _ptr(lse2), _ptr(dq_acc), _ptr(dkdv),
+            _ptr(dq), _ptr(dk), _ptr(dv), B, S, Hq, k.shape[2], D, DTYPE_CODES[q.dtype], ctypes.byref(args),
+            _ptr(dq_order), _ptr(status), _stream(stream, q))
+    _check(rc, "rfa_scored_bwd_local", kernels=3)
 
 
 def bwd_hop_noalloc(q, k, v, dout, lse2, delta, dq, dkdv_prev, dkdv_out, softmax_scale: float,

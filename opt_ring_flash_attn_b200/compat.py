@@ -2,8 +2,8 @@
 ring_flash_attn.py:385-463), so that callers of ``ring_flash_attn_func`` / ``_kvpacked_func`` /
 ``_qkvpacked_func`` can switch without code changes.
 
-Only what this build computes is accepted: dropout 0, no sliding window, no ALiBi.  Anything else raises
-``NotImplementedError`` instead of being silently ignored.  ``return_attn_probs=True`` returns
+Only what this build computes is accepted: dropout 0, no sliding window.  Anything else raises ``NotImplementedError``
+instead of being silently ignored.  ``alibi_slopes`` (fp32 ``[H_q]`` or ``[B, H_q]``) go to :func:`scored_flash_attn`.  ``return_attn_probs=True`` returns
 ``(out, softmax_lse, None)`` like the reference (ring_flash_attn.py:362).  ``deterministic=True``
 (ring_flash_attn.py:179, 245) selects the ordered dQ reductions: gradients are bit-reproducible run to run.
 """
@@ -13,22 +13,24 @@ import contextlib
 
 from .api import deterministic as _deterministic
 from .api import ring_flash_attn, ring_flash_attn_with_lse
+from .scored import scored_flash_attn_with_lse
 
 
-def _check_unsupported(dropout_p, window_size, alibi_slopes):
+def _check_unsupported(dropout_p, window_size):
     if dropout_p != 0.0:
         raise NotImplementedError("dropout_p != 0 is not supported")
     if tuple(window_size) != (-1, -1):
         raise NotImplementedError("sliding-window attention is not supported")
-    if alibi_slopes is not None:
-        raise NotImplementedError("ALiBi is not supported")
 
 
 def ring_flash_attn_func(q, k, v, dropout_p=0.0, softmax_scale=None, causal=False, window_size=(-1, -1),
                          alibi_slopes=None, deterministic=False, return_attn_probs=False, group=None):
-    _check_unsupported(dropout_p, window_size, alibi_slopes)
+    _check_unsupported(dropout_p, window_size)
     # False leaves the surrounding default (context manager or RFA_B200_DETERMINISTIC) in force
     with (_deterministic(True) if deterministic else contextlib.nullcontext()):
+        if alibi_slopes is not None:
+            out, lse = scored_flash_attn_with_lse(q, k, v, softmax_scale, causal, alibi_slopes=alibi_slopes, group=group)
+            return (out, lse, None) if return_attn_probs else out
         if return_attn_probs:
             out, lse = ring_flash_attn_with_lse(q, k, v, softmax_scale=softmax_scale, causal=causal, group=group)
             return out, lse, None

@@ -1,0 +1,694 @@
+// Forward hop of attention with modified scores: capped by a tanh, biased by distance, masked by documents and prefixes.
+//
+//   x = scale * q.k;   y = cap * tanh(x / cap);   z = y - slope |i - j|;   O, lse = online softmax over the visible keys
+//
+// The structure of a CTA is that of the plain forward hop (a TMA warp, an issuing warp, one softmax warpgroup per tile of
+// 128 queries; tensor memory holds O and the scores), with these differences.
+//  * A CTA walks the range of key tiles that the hull of its rows' intervals gives, each of its query tiles its own part of
+//    it, so what no row sees is neither loaded nor multiplied.  With a mask the blocks take their tiles from its work list,
+//    long ones first.
+//  * Scores are brought to log2 units before the row maximum is taken, where a cap or a bias stands between them and it.
+//  * A tile inside every row's interval needs no test; in the others a row compares the key with its own interval.
+//  * A row that has seen no key keeps the finite maximum kNoKey, and ends with out = 0, lse = -inf.
+//  * The issuing warp clears the padding rows of a V tile that holds the border between real rows and padding.
+#include "fwd_common.cuh"
+#include "scored.cuh"
+
+namespace rfa {
+
+struct ScoredFwdParams {
+  float* acc;
+  float* m;
+  float* l;
+  void* out;
+  float* lse;
+  int B, S, Hq, Hkv, D;
+  int Spad, nT;
+  int first, last;
+  int* status;
+  ScoreParams sc;
+};
+
+// Scores of 32 keys in log2 units: the cap and the bias.  `bias` holds what is added to the first two keys, `step` what it
+// grows by from pair to pair (bias and step include the constant of the tanh).
+template <int kKind>
+__device__ __forceinline__ void transform32(uint32_t (&r)[32], uint64_t scale2, uint64_t gain2, uint64_t bias, uint64_t step) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    uint64_t y;
+    if constexpr (kKind == 1) {
+      y = fma2(pack_u2(r[2 * i], r[2 * i + 1]), scale2, bias);
+    } else {
+      // cap * tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1); scale2 turns the raw score into the exponent, gain2 is
+      // -2 cap, cap itself is in the bias.  Both ends of the range come out as they should: exp2 gives 0 or an infinity.
+      float a0, a1;
+      unpack_f2(mul2(pack_u2(r[2 * i], r[2 * i + 1]), scale2), a0, a1);
+      float e0, e1;
+      unpack_f2(add2(pack_f2(fast_exp2(a0), fast_exp2(a1)), pack_f2(1.f, 1.f)), e0, e1);
+      y = fma2(pack_f2(fast_rcp(e0), fast_rcp(e1)), gain2, bias);
+    }
+    unpack_u2(y, r[2 * i], r[2 * i + 1]);
+    bias = add2(bias, step);
+  }
+}
+
+template <int DP, int BN, int NQ, int NS, typename T, int kKind>
+__global__ void __launch_bounds__(128 + NQ * 128, 1)
+    scored_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                      const __grid_constant__ CUtensorMap tm_v, const ScoredFwdParams p) {
+  using Cfg = FwdCfg<DP, BN, NQ, NS>;
+  constexpr int kSlots = Cfg::kSlots;
+  constexpr bool kBf16 = Pack2<T>::kIsBf16;
+  constexpr int kPvParts = (DP == 64) ? 2 : 4;     // P is handed to the issuer in parts, as in the plain hop
+  constexpr int kPartChunks = BN / 32 / kPvParts;
+  constexpr int kPolyEvery = (NQ == 2) ? kFwdPolyEvery : 0;
+
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t bar_q_full;
+  __shared__ uint64_t bar_kv_full[kSlots];
+  __shared__ uint64_t bar_kv_empty[kSlots];
+  __shared__ uint64_t bar_s_full[NQ * NS];
+  __shared__ uint64_t bar_p_ready[NQ * NS * kPvParts];
+  __shared__ uint64_t bar_pv_done[NQ];
+  __shared__ uint32_t tmem_holder;
+  __shared__ int abort_flag, skip_flag;
+
+  const int tid = threadIdx.x;
+  const int warp = tid >> 5;
+  const int lane = tid & 31;
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t s_q = smem_base;
+  const uint32_t s_kv = smem_base + NQ * Cfg::kQBytes;
+
+  if (tid == 0) {
+    abort_flag = 0;
+    mbar_init(&bar_q_full, 1);
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&bar_kv_full[i], 1);
+      mbar_init(&bar_kv_empty[i], 1);
+    }
+    for (int i = 0; i < NQ * NS; ++i) {
+      mbar_init(&bar_s_full[i], 1);
+      for (int h = 0; h < kPvParts; ++h) mbar_init(&bar_p_ready[i * kPvParts + h], 128);
+    }
+    for (int i = 0; i < NQ; ++i) mbar_init(&bar_pv_done[i], 1);
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&tmem_holder, 512);
+    tmem_relinquish();
+  }
+  pdl_wait();  // nothing above touches global memory
+
+  // ---- tile coordinates: most work first, heads fastest ----
+  const int nQs = (p.nT + NQ - 1) / NQ;
+  int b, h, qs;
+  if (p.sc.has_mask) {
+    const int item = __ldg((NQ == 2 ? p.sc.mask.order_q2 : p.sc.mask.order_q) + blockIdx.x / p.Hq);
+    h = blockIdx.x % p.Hq;
+    b = item / nQs;
+    qs = item % nQs;
+  } else {
+    const int per_qs = p.Hq * p.B, rem = static_cast<int>(blockIdx.x) % per_qs;
+    qs = nQs - 1 - static_cast<int>(blockIdx.x) / per_qs;
+    b = rem / p.Hq;
+    h = rem % p.Hq;
+  }
+  const int hkv = h / (p.Hq / p.Hkv);
+
+  // Range of key tiles of each query tile: tiles [j0 + t_lo[q], j0 + t_hi[q]) of the block, j0 the first of the CTA.
+  int m0[NQ], t_lo[NQ], t_hi[NQ], full_lo[NQ], full_hi[NQ];  // keys [full_lo, full_hi) of the block are seen by every row
+  int j0 = INT_MAX, j1 = 0;
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    m0[q] = (qs * NQ + q) * 128;
+    t_lo[q] = t_hi[q] = full_lo[q] = full_hi[q] = 0;
+    if (m0[q] < p.S) {
+      const int4 hull = query_hull(p.sc, b, p.nT, qs * NQ + q, p.S);
+      const int lo = max(hull.x - p.sc.k_pos, 0), hi = min(hull.w - p.sc.k_pos, p.S);
+      full_lo[q] = max(hull.y, p.sc.k_pos) - p.sc.k_pos;
+      full_hi[q] = min(hull.z - p.sc.k_pos, p.S);
+      if (lo < hi) {
+        t_lo[q] = lo / BN;
+        t_hi[q] = (hi + BN - 1) / BN;
+        j0 = min(j0, t_lo[q]);
+        j1 = max(j1, t_hi[q]);
+      }
+    }
+  }
+  if (j0 > j1) j0 = j1;  // nothing to do
+  const int nmax = j1 - j0;
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    t_lo[q] = t_hi[q] > 0 ? t_lo[q] - j0 : 0;
+    t_hi[q] = t_hi[q] > 0 ? t_hi[q] - j0 : 0;
+  }
+  // rows of the key block that are no padding
+  const int real_lo = p.sc.has_mask ? __ldg(p.sc.mask.real + 2 * b) - p.sc.k_pos : 0;
+  const int real_hi = p.sc.has_mask ? __ldg(p.sc.mask.real + 2 * b + 1) - p.sc.k_pos : p.S;
+
+  if (tid == 0) skip_flag = *reinterpret_cast<volatile int*>(p.status);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = tmem_holder;
+  if (skip_flag != 0) {  // an earlier kernel gave up
+    if (warp == 0) tmem_dealloc(tmem_base, 512);
+    return;
+  }
+  volatile int* abort_p = &abort_flag;
+
+  if (warp < 4) {
+    if constexpr (NQ == 2) setmaxnreg_dec<Cfg::kServiceRegs>();
+    if (warp == 0) {
+      // =========================== TMA producer ===========================
+      if (lane == 0 && nmax > 0) {
+        tma_prefetch_desc(&tm_q);
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
+        int nvalid = 0;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) nvalid += (t_hi[q] > 0) ? 1 : 0;
+        mbar_expect_tx(&bar_q_full, static_cast<uint32_t>(nvalid) * Cfg::kQBytes);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          if (t_hi[q] > 0) {
+#pragma unroll
+            for (int pn = 0; pn < Cfg::kPanels; ++pn)
+              tma_load_4d(s_q + q * Cfg::kQBytes + pn * (128 * 128), &tm_q, &bar_q_full, pn * 64, h, m0[q], b);
+          }
+        }
+        SlotWalk<kSlots> w;
+        auto load = [&](int which, int j) {
+#pragma unroll
+          for (int pc = 0; pc < Cfg::kPieces; ++pc, w.next()) {
+            if (!mbar_wait(&bar_kv_empty[w.slot], w.phase ^ 1, abort_p)) return false;
+            mbar_expect_tx(&bar_kv_full[w.slot], Cfg::kKVBytes);
+#pragma unroll
+            for (int pn = 0; pn < Cfg::kPanels / Cfg::kPieces; ++pn)
+              tma_load_4d(s_kv + w.slot * Cfg::kKVBytes + pn * (BN * 128), which ? &tm_v : &tm_k, &bar_kv_full[w.slot],
+                          (Cfg::kPanels / Cfg::kPieces * pc + pn) * 64, hkv, (j0 + j) * BN, b);
+          }
+          return true;
+        };
+        if constexpr (NS == 2) {  // in the order in which the products use them: K0, K1, V0, K2, V1, ...
+          bool ok = load(0, 0);
+          for (int j = 0; j < nmax && ok; ++j) ok = (j + 1 == nmax || load(0, j + 1)) && load(1, j);
+        } else {
+          bool ok = true;
+          for (int j = 0; j < nmax && ok; ++j) ok = load(0, j) && load(1, j);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 1 && nmax > 0) {
+      // =========================== MMA issuer ===========================
+      const uint32_t el = elect_one();
+      const int d16 = (p.D + 15) / 16 * 16;
+      constexpr uint32_t idesc_qk = make_idesc(128, BN, kBf16, false, false);
+      // A tile on the border between real rows and padding: what its products would multiply by 0 is cleared first.
+      auto clear_v = [&](int slot, int j) {
+        const int r0 = (j0 + j) * BN;
+        if (real_lo > r0 || real_hi < min(r0 + BN, p.S))
+          clear_padding_rows(s_kv + slot * Cfg::kKVBytes, Cfg::kPanels / Cfg::kPieces, BN, real_lo - r0, real_hi - r0, lane);
+      };
+      if constexpr (NS == 2) {
+        auto idesc_pv = [&](int pc) { return make_idesc(128, min(d16 - pc * 128, 128), kBf16, false, true); };
+        const uint32_t q_lo = desc_lo_kmajor(s_q);
+        SlotWalk<kSlots> w;
+        auto s_tm = [&](int j) { return tmem_base + Cfg::kTmS + (j & 1) * BN; };
+        auto qk = [&](int j) {
+          bool got = true;
+          static_for<0, Cfg::kPieces>([&](auto pc_) {
+            constexpr int pc = decltype(pc_)::value;
+            if (!got) return;
+            got = mbar_wait_warp(&bar_kv_full[w.slot], w.phase, abort_p);
+            if (!got) return;
+            tc_fence_after_sync();
+            issue_qk<128, BN>(s_tm(j), q_lo + pc * (2 * 128 * 128 / 16), desc_lo_kmajor(s_kv + w.slot * Cfg::kKVBytes),
+                              idesc_qk, el, pc > 0);
+            mma_commit_e(&bar_kv_empty[w.slot], el);
+            w.next();
+          });
+          if (got) mma_commit_e(&bar_s_full[j & 1], el);
+          return got;
+        };
+        bool ok = mbar_wait_warp(&bar_q_full, 0, abort_p) && qk(0);
+        for (int j = 0; j < nmax && ok; ++j) {
+          // Score buffer (j+1)&1 is free: P_{j-1} was consumed by the PV issued last iteration.
+          if (j + 1 < nmax && !qk(j + 1)) break;
+          uint32_t v_lo[Cfg::kPieces];
+          int v_slot[Cfg::kPieces];
+#pragma unroll
+          for (int pc = 0; pc < Cfg::kPieces; ++pc, w.next()) {
+            v_slot[pc] = w.slot;
+            v_lo[pc] = desc_lo_mnmajor(s_kv + w.slot * Cfg::kKVBytes, BN * 128);
+            ok = ok && mbar_wait_warp(&bar_kv_full[w.slot], w.phase, abort_p);
+            if (ok) clear_v(w.slot, j);
+          }
+          static_for<0, kPvParts>([&](auto h_) {
+            constexpr int h = decltype(h_)::value;
+            ok = ok && mbar_wait_warp(&bar_p_ready[(j & 1) * kPvParts + h], (j >> 1) & 1, abort_p);
+            if (!ok) return;
+            tc_fence_after_sync();
+#pragma unroll
+            for (int pc = 0; pc < Cfg::kPieces; ++pc)
+              issue_pv<128, BN, 2 * kPartChunks * h, 2 * kPartChunks * (h + 1)>(
+                  tmem_base + Cfg::kTmO + pc * 128, s_tm(j), v_lo[pc], idesc_pv(pc), (h > 0) || (j > 0) || (p.first == 0), el);
+          });
+          if (!ok) break;
+          mma_commit_e(&bar_pv_done[0], el);
+#pragma unroll
+          for (int pc = 0; pc < Cfg::kPieces; ++pc) mma_commit_e(&bar_kv_empty[v_slot[pc]], el);
+        }
+      } else {
+        const uint32_t idesc_pv = make_idesc(128, d16, kBf16, false, true);
+        auto slot_of = [&](int u) { return u % kSlots; };
+        auto par_of = [&](int u) { return static_cast<uint32_t>((u / kSlots) & 1); };
+        auto k_lo = [&](int u) { return desc_lo_kmajor(s_kv + slot_of(u) * Cfg::kKVBytes); };
+        auto v_lo = [&](int u) { return desc_lo_mnmajor(s_kv + slot_of(u) * Cfg::kKVBytes, BN * 128); };
+        uint32_t q_lo[NQ];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) q_lo[q] = desc_lo_kmajor(s_q + q * Cfg::kQBytes);
+        auto s_tm = [&](int q) { return tmem_base + Cfg::kTmS + q * BN; };
+        auto o_tm = [&](int q) { return tmem_base + Cfg::kTmO + q * DP; };
+        auto wait_tile = [&](int u) { return mbar_wait_warp(&bar_kv_full[slot_of(u)], par_of(u), abort_p); };
+        bool ok = mbar_wait_warp(&bar_q_full, 0, abort_p) && wait_tile(0);
+        if (ok) {
+          tc_fence_after_sync();
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            if (t_lo[q] == 0 && t_hi[q] > 0) {
+              issue_qk<DP, BN>(s_tm(q), q_lo[q], k_lo(0), idesc_qk, el);
+              mma_commit_e(&bar_s_full[q], el);
+            }
+          }
+          mma_commit_e(&bar_kv_empty[slot_of(0)], el);
+        }
+        for (int j = 0; j < nmax && ok; ++j) {
+          const int uv = 2 * j + 1, uk = 2 * (j + 1);
+          if (!wait_tile(uv)) break;
+          clear_v(slot_of(uv), j);
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            if (j >= t_lo[q] && j < t_hi[q]) {
+              static_for<0, kPvParts>([&](auto h_) {
+                constexpr int h = decltype(h_)::value;
+                if (ok) {
+                  if (!mbar_wait_warp(&bar_p_ready[q * kPvParts + h], (j - t_lo[q]) & 1, abort_p)) {
+                    ok = false;
+                  } else {
+                    tc_fence_after_sync();
+                    issue_pv<DP, BN, 2 * kPartChunks * h, 2 * kPartChunks * (h + 1)>(
+                        o_tm(q), s_tm(q), v_lo(uv), idesc_pv, (h > 0) || (j > t_lo[q]) || (p.first == 0), el);
+                  }
+                }
+              });
+              if (!ok) break;
+              if (j + 1 == t_hi[q]) mma_commit_e(&bar_pv_done[q], el);
+            }
+            if (j + 1 >= t_lo[q] && j + 1 < t_hi[q]) {
+              if (!wait_tile(uk)) { ok = false; break; }
+              tc_fence_after_sync();
+              issue_qk<DP, BN>(s_tm(q), q_lo[q], k_lo(uk), idesc_qk, el);
+              mma_commit_e(&bar_s_full[q], el);
+            }
+          }
+          if (!ok) break;
+          mma_commit_e(&bar_kv_empty[slot_of(uv)], el);
+          if (j + 1 < nmax) {
+            if (!wait_tile(uk)) break;  // also where no query tile uses it: a slot is released only once it is filled
+            mma_commit_e(&bar_kv_empty[slot_of(uk)], el);
+          }
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    // =========================== softmax warpgroups ===========================
+    if constexpr (NQ == 2) setmaxnreg_inc<Cfg::kSoftmaxRegs>();
+    const int q = (warp - 4) >> 2;
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    // selected, not indexed: an array indexed at run time would live in local memory for the issuer as well
+    const bool second = NQ == 2 && q == 1;
+    const int t_first = second ? t_lo[NQ - 1] : t_lo[0];
+    const int n = (second ? t_hi[NQ - 1] : t_hi[0]) - t_first;
+    const int m0_q = second ? m0[NQ - 1] : m0[0];
+    const int full_lo_q = second ? full_lo[NQ - 1] : full_lo[0];
+    const int full_hi_q = second ? full_hi[NQ - 1] : full_hi[0];
+    const int n_c32 = (p.D + 31) / 32;
+    const int row_g = m0_q + row;
+    const uint32_t o_addr = tmem_base + lane_addr + Cfg::kTmO + q * DP;
+    const size_t bh = static_cast<size_t>(b) * p.Hq + h;
+    float* acc_tile = p.acc + ((bh * p.nT + (qs * NQ + q)) * (DP / 4)) * 512;  // [DP/4][128][4]
+    const size_t ml_idx = bh * p.Spad + row_g;
+
+    if (m0_q < p.S && !(n == 0 && !p.first && !p.last)) {
+      bool ok = true;
+      float m_used = kNoKey;
+      float l_sum = 0.f;
+      if (!p.first || n == 0) {  // the state of the hops before, or of none
+        if (!p.first) {
+          m_used = p.m[ml_idx];
+          l_sum = p.l[ml_idx];
+        }
+#pragma unroll 1
+        for (int c = 0; c < n_c32; ++c) {
+          uint32_t r[32];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (!p.first) v = *reinterpret_cast<const float4*>(acc_tile + ((c * 8 + k) * 128 + row) * 4);
+            r[4 * k + 0] = __float_as_uint(v.x);
+            r[4 * k + 1] = __float_as_uint(v.y);
+            r[4 * k + 2] = __float_as_uint(v.z);
+            r[4 * k + 3] = __float_as_uint(v.w);
+          }
+          tmem_st32(o_addr + c * 32, r);
+        }
+        tmem_st_wait();
+      }
+      // Keys of the block that this row sees: [lo, lo + width).
+      int lo = 0, width = p.S;
+      if (row_g < p.S) {
+        int hi = p.S;
+        if (p.sc.has_mask) {
+          const size_t at = static_cast<size_t>(b) * p.sc.len + p.sc.q_pos + row_g;
+          lo = max(__ldg(p.sc.mask.q_lo + at) - p.sc.k_pos, 0);
+          hi = min(__ldg(p.sc.mask.q_hi + at) - p.sc.k_pos, p.S);
+        } else if (p.sc.causal) {
+          hi = min(p.sc.q_pos + row_g + 1 - p.sc.k_pos, p.S);
+        }
+        width = max(hi - lo, 0);
+      }
+      const Exp2Poly exp2_poly;
+      const float scale_log2 = p.sc.scale * kLog2e;
+      const float cap_log2 = p.sc.cap * kLog2e;
+      const float slope = kKind > 0 ? slope_log2(p.sc, b, p.Hq, h) : 0.f;
+      const int ahead = p.sc.q_pos + row_g - p.sc.k_pos;  // position of this row, from the first key of the block
+      // what a raw score is multiplied by, and the tanh's -2 cap
+      const float in_scale = kKind == 2 ? 2.f * scale_log2 / p.sc.cap : scale_log2;
+
+#pragma unroll 1
+      for (int j = 0; j < n; ++j) {
+        const int sb = (NS == 2) ? (j & 1) : 0;
+        const uint32_t par = (NS == 2) ? ((j >> 1) & 1) : (j & 1);
+        if (!mbar_wait_warp(&bar_s_full[q * NS + sb], par, abort_p)) { ok = false; break; }
+        tc_fence_after_sync();
+        const uint32_t s_addr = tmem_base + lane_addr + Cfg::kTmS + (q * NS + sb) * BN;
+        const int n0 = (j0 + t_first + j) * BN;
+        const bool masked = n0 < full_lo_q || n0 + BN > full_hi_q;
+
+        constexpr int NCH = BN / 32;
+        uint32_t r[NCH][32];
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) tmem_ld32(s_addr + c * 32, r[c]);
+        tmem_ld_wait32(r[0]);
+#pragma unroll
+        for (int c = 1; c < NCH; ++c) reg_fence32(r[c]);
+        if constexpr (kKind > 0) {
+          // Keys all before or all after the queries: the distance is linear in the key, sign * (ahead - key).
+          const int d0 = p.sc.q_pos + m0_q - p.sc.k_pos;  // of the first row
+          const bool before = n0 + BN - 1 <= d0, after = n0 >= d0 + 127;
+          const float sign_slope = before ? slope : after ? -slope : 0.f;
+          const uint64_t step = pack_f2(2.f * sign_slope, 2.f * sign_slope);
+          const uint64_t in2 = pack_f2(in_scale, in_scale);
+          const uint64_t gain2 = pack_f2(-2.f * cap_log2, -2.f * cap_log2);
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) {
+            const float b0 = fmaf(static_cast<float>(n0 + c * 32 - ahead), sign_slope, kKind == 2 ? cap_log2 : 0.f);
+            transform32<kKind>(r[c], in2, gain2, pack_f2(b0, b0 + sign_slope), step);
+          }
+          if (!before && !after && slope != 0.f) {
+            const float d = static_cast<float>(ahead - n0);
+#pragma unroll
+            for (int c = 0; c < NCH; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                r[c][i] = __float_as_uint(fmaf(-slope, fabsf(d - static_cast<float>(c * 32 + i)), __uint_as_float(r[c][i])));
+          }
+        }
+        if (masked) {
+          const int base = n0 - lo;
+#pragma unroll
+          for (int c = 0; c < NCH; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (static_cast<unsigned>(base + c * 32 + i) >= static_cast<unsigned>(width))
+                r[c][i] = __float_as_uint(-INFINITY);
+        }
+        // row maximum (independent partial maxima keep the dependency chains short)
+        float mxp[NCH][2];
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+          mxp[c][0] = __uint_as_float(r[c][0]);
+          mxp[c][1] = __uint_as_float(r[c][1]);
+#pragma unroll
+          for (int i = 2; i < 30; i += 4) {
+            mxp[c][0] = max3_nan(mxp[c][0], __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
+            mxp[c][1] = max3_nan(mxp[c][1], __uint_as_float(r[c][i + 2]), __uint_as_float(r[c][i + 3]));
+          }
+          mxp[c][0] = max3_nan(mxp[c][0], __uint_as_float(r[c][30]), __uint_as_float(r[c][31]));
+        }
+        float mx = max_nan(mxp[0][0], mxp[0][1]);
+#pragma unroll
+        for (int c = 1; c < NCH; ++c) mx = max3_nan(mx, mxp[c][0], mxp[c][1]);
+        const float m_new = max_nan(m_used, kKind == 0 ? mx * scale_log2 : mx);
+
+        // lazy rescale: only when the maximum grew by more than 2^8, or is no number
+        bool need;
+        if (j == 0 && p.first) {
+          m_used = m_new;
+          need = false;
+        } else {
+          need = !(m_new - m_used <= 8.0f);
+        }
+        if (__any_sync(0xffffffffu, need)) {
+          const float alpha = need ? fast_exp2(m_used - m_new) : 1.0f;
+          if (need) m_used = m_new + (m_new - m_new);
+          l_sum *= alpha;
+          // With one score buffer the arrival on bar_s_full that let this iteration start was committed after
+          // O += P_{j-1} V_{j-1} was issued, so that product has retired; with two buffers it has its own barrier.
+          if (NS == 2 && j > 0) {
+            if (!mbar_wait_warp(&bar_pv_done[q], (j - 1) & 1, abort_p)) { ok = false; break; }
+            tc_fence_after_sync();
+          }
+#pragma unroll 1
+          for (int c = 0; c < 2 * n_c32; ++c) {
+            uint32_t o16[16];
+            tmem_ld16(o_addr + c * 16, o16);
+            tmem_ld_wait16(o16);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o16[i] = __float_as_uint(__uint_as_float(o16[i]) * alpha);
+            tmem_st16(o_addr + c * 16, o16);
+          }
+          tmem_st_wait();
+        }
+
+        // P = exp2(z - m_used), packed to 16 bit over the start of S (rounded for the product, as in the plain hop; the sum
+        // is taken before).  The polynomial gives a masked key 2^-125 where exp2 gives 0: beside a real key nothing.
+        const uint64_t scale2 = pack_f2(scale_log2, scale_log2);
+        const uint64_t negm2 = pack_f2(-m_used, -m_used);
+        uint64_t lp2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+          uint32_t u[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t s2 = pack_u2(r[c][2 * i], r[c][2 * i + 1]);
+            const uint64_t x2 = kKind == 0 ? fma2(s2, scale2, negm2) : add2(s2, negm2);
+            uint64_t p2;
+            float p0, p1;
+            if (kPolyEvery > 0 && (i % (kPolyEvery > 0 ? kPolyEvery : 1)) == kPolyEvery - 1) {
+              p2 = exp2_poly(x2);
+              unpack_f2(p2, p0, p1);
+            } else {
+              float x0, x1;
+              unpack_f2(x2, x0, x1);
+              p0 = fast_exp2(x0);
+              p1 = fast_exp2(x1);
+              p2 = pack_f2(p0, p1);
+            }
+            lp2[i & 1] = add2(lp2[i & 1], p2);
+            u[i] = Pack2<T>::pack(p0, p1);
+          }
+          if (c > 0 && c % kPartChunks == 0) {
+            // the previous part of P has landed: the issuer may start O += P V on them
+            tmem_st_wait();
+            tc_fence_before_sync();
+            mbar_arrive(&bar_p_ready[(q * NS + sb) * kPvParts + c / kPartChunks - 1]);
+          }
+          tmem_st16(s_addr + c * 16, u);
+        }
+        tmem_st_wait();
+        tc_fence_before_sync();
+        mbar_arrive(&bar_p_ready[(q * NS + sb) * kPvParts + kPvParts - 1]);
+        {
+          float a0, a1, b0, b1;
+          unpack_f2(lp2[0], a0, a1);
+          unpack_f2(lp2[1], b0, b1);
+          l_sum += (a0 + a1) + (b0 + b1);
+        }
+      }
+
+      // ---- epilogue: wait for the last PV, then spill state or write the result ----
+      // With two score buffers the last scores only prove that O += P_{n-3} V_{n-3} has retired: a wait for the parity of
+      // the last product alone would also be satisfied by the phase before the one of tile n-2.
+      if (NS == 2 && ok && n > 1) ok = mbar_wait_warp(&bar_pv_done[q], (n - 2) & 1, abort_p);
+      if (ok && n > 0) ok = mbar_wait_warp(&bar_pv_done[q], (NS == 2) ? ((n - 1) & 1) : 0, abort_p);
+      if (ok) {
+        tc_fence_after_sync();
+        l_sum += m_used - m_used;  // nothing, or NaN
+        if (p.last) {
+          const bool empty = m_used == kNoKey;
+          const float inv = 1.0f / l_sum;
+          const bool row_ok = row_g < p.S;
+          T* orow = reinterpret_cast<T*>(p.out) + ((static_cast<size_t>(b) * p.S + row_g) * p.Hq + h) * p.D;
+#pragma unroll 1
+          for (int c = 0; c < n_c32; ++c) {
+            uint32_t r[32];
+            tmem_ld32(o_addr + c * 32, r);
+            tmem_ld_wait32(r);
+            if (row_ok) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if (c * 32 + k * 8 < p.D) {
+                  uint4 w;
+                  w.x = Pack2<T>::pack(__uint_as_float(r[8 * k + 0]) * inv, __uint_as_float(r[8 * k + 1]) * inv);
+                  w.y = Pack2<T>::pack(__uint_as_float(r[8 * k + 2]) * inv, __uint_as_float(r[8 * k + 3]) * inv);
+                  w.z = Pack2<T>::pack(__uint_as_float(r[8 * k + 4]) * inv, __uint_as_float(r[8 * k + 5]) * inv);
+                  w.w = Pack2<T>::pack(__uint_as_float(r[8 * k + 6]) * inv, __uint_as_float(r[8 * k + 7]) * inv);
+                  if (empty) w = make_uint4(0, 0, 0, 0);
+                  *reinterpret_cast<uint4*>(orow + c * 32 + k * 8) = w;
+                }
+              }
+            }
+          }
+          if (row_ok) p.lse[ml_idx] = empty ? -INFINITY : (m_used + log2f(l_sum)) * 0.6931471805599453f;
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < n_c32; ++c) {
+            uint32_t r[32];
+            tmem_ld32(o_addr + c * 32, r);
+            tmem_ld_wait32(r);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              float4 v;
+              v.x = __uint_as_float(r[4 * k + 0]);
+              v.y = __uint_as_float(r[4 * k + 1]);
+              v.z = __uint_as_float(r[4 * k + 2]);
+              v.w = __uint_as_float(r[4 * k + 3]);
+              *reinterpret_cast<float4*>(acc_tile + ((c * 8 + k) * 128 + row) * 4) = v;
+            }
+          }
+          p.m[ml_idx] = m_used;
+          p.l[ml_idx] = l_sum;
+        }
+      }
+    }
+    __syncwarp();
+  }
+
+  // ---- teardown: every role arrives here, also after an abort ----
+  tc_fence_before_sync();
+  __syncthreads();
+  if (abort_flag) {
+    // Give copies that are still in flight time to land before the CTA's shared memory is released.
+    const unsigned long long t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+    if (tid == 0) atomicExch(p.status, kStatusWaitTimeout);
+  }
+  if (warp == 0) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+template <int DP, int BN, int NQ, int NS, typename T, int kKind>
+static int launch_scored_fwd(const void* q, const void* k, const void* v, const ScoredFwdParams& prm, int dtype,
+                             cudaStream_t stream) {
+  using Cfg = FwdCfg<DP, BN, NQ, NS>;
+  CUtensorMap tq, tk, tv;
+  int rc;
+  if ((rc = make_tmap_bshd(&tq, q, dtype, prm.B, prm.S, prm.Hq, prm.D, 128)) != RFA_OK) return rc;
+  if ((rc = make_tmap_bshd(&tk, k, dtype, prm.B, prm.S, prm.Hkv, prm.D, BN)) != RFA_OK) return rc;
+  if ((rc = make_tmap_bshd(&tv, v, dtype, prm.B, prm.S, prm.Hkv, prm.D, BN)) != RFA_OK) return rc;
+  auto kern = scored_fwd_kernel<DP, BN, NQ, NS, T, kKind>;
+  static bool attr_done[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) { cudaGetLastError(); return RFA_ERR_CUDA; }
+  if (!attr_done[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    if (e != cudaSuccess) { cudaGetLastError(); return RFA_ERR_CUDA; }
+    if (NQ == 2) {
+      // A raise that the launch's pool (threads x registers per thread) cannot satisfy would wait forever: a build whose
+      // register count does not cover the allowances is refused.
+      cudaFuncAttributes fa;
+      e = cudaFuncGetAttributes(&fa, kern);
+      if (e != cudaSuccess) { cudaGetLastError(); return RFA_ERR_CUDA; }
+      if (fa.numRegs * Cfg::kThreads < Cfg::kPoolRegs) return RFA_ERR_UNSUPPORTED;
+    }
+    attr_done[dev] = true;
+  }
+  const unsigned grid = static_cast<unsigned>((prm.nT + NQ - 1) / NQ) * prm.Hq * prm.B;
+  return launch_chained(kern, grid, Cfg::kThreads, Cfg::kSmemBytes, stream, tq, tk, tv, prm);
+}
+
+template <typename T, int kKind>
+static int dispatch_scored_fwd(const void* q, const void* k, const void* v, const ScoredFwdParams& prm, int dtype,
+                               cudaStream_t stream) {
+  switch (padded_head_dim(prm.D)) {
+    case 64: return launch_scored_fwd<64, 128, 2, 1, T, kKind>(q, k, v, prm, dtype, stream);
+    case 128: return launch_scored_fwd<128, 128, 2, 1, T, kKind>(q, k, v, prm, dtype, stream);
+    case 256: return launch_scored_fwd<256, 128, 1, 2, T, kKind>(q, k, v, prm, dtype, stream);
+    default: return RFA_ERR_UNSUPPORTED;
+  }
+}
+
+template <typename T>
+static int dispatch_scored_kind(const void* q, const void* k, const void* v, const ScoredFwdParams& prm, int dtype,
+                                cudaStream_t stream) {
+  switch (score_kind(prm.sc)) {
+    case 0: return dispatch_scored_fwd<T, 0>(q, k, v, prm, dtype, stream);
+    case 1: return dispatch_scored_fwd<T, 1>(q, k, v, prm, dtype, stream);
+    default: return dispatch_scored_fwd<T, 2>(q, k, v, prm, dtype, stream);
+  }
+}
+
+}  // namespace rfa
+
+extern "C" int rfa_scored_fwd_hop(const void* q, const void* k, const void* v, float* acc, float* m, float* l, void* out,
+                                  float* lse, int B, int S, int Hq, int Hkv, int D, int dtype, const rfa_score_args* args,
+                                  int first, int last, int* status, void* stream) {
+  using namespace rfa;
+  if (!q || !k || !v || !status) return RFA_ERR_INVALID_ARG;
+  if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0) return RFA_ERR_INVALID_ARG;
+  if (!(first && last) && (!acc || !m || !l)) return RFA_ERR_INVALID_ARG;
+  if (last && (!out || !lse)) return RFA_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(acc) & 15u) || (reinterpret_cast<uintptr_t>(out) & 15u)) return RFA_ERR_INVALID_ARG;
+  if (padded_head_dim(D) == 0) return RFA_ERR_UNSUPPORTED;
+  if (dtype != RFA_DTYPE_BF16 && dtype != RFA_DTYPE_FP16) return RFA_ERR_UNSUPPORTED;
+  ScoredFwdParams prm;
+  const int rc = make_score_params(args, B, S, &prm.sc);
+  if (rc != RFA_OK) return rc;
+  prm.acc = acc;
+  prm.m = m;
+  prm.l = l;
+  prm.out = out;
+  prm.lse = lse;
+  prm.B = B;
+  prm.S = S;
+  prm.Hq = Hq;
+  prm.Hkv = Hkv;
+  prm.D = D;
+  prm.Spad = round_up(S, 128);
+  prm.nT = prm.Spad / 128;
+  prm.first = first ? 1 : 0;
+  prm.last = last ? 1 : 0;
+  prm.status = status;
+  if (static_cast<long long>(prm.nT) * Hq * B > INT_MAX) return RFA_ERR_TOO_LARGE;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == RFA_DTYPE_BF16) return dispatch_scored_kind<__nv_bfloat16>(q, k, v, prm, dtype, s);
+  return dispatch_scored_kind<__half>(q, k, v, prm, dtype, s);
+}

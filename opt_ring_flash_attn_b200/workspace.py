@@ -101,8 +101,29 @@ def _retire(ws) -> None:
     ws.comms.clear()
 
 
+# device -> status word of the operators that allocate their scratch per call (any number of streams may use it: a kernel
+# writes it only where it fails)
+_status_cache: Dict[torch.device, ForwardWorkspace] = {}
+
+
 def all_workspaces() -> List:
-    return [ws for _, ws in list(_fwd_cache.values()) + list(_bwd_cache.values())]
+    return [ws for _, ws in list(_fwd_cache.values()) + list(_bwd_cache.values())] + list(_status_cache.values())
+
+
+def status_workspace(device: torch.device) -> ForwardWorkspace:
+    """The status word of a device, with its pinned copy.  The first use must not be inside a graph capture."""
+    ws = _status_cache.get(device)
+    if ws is None:
+        if device.type == "cuda":
+            with torch.cuda.device(device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the first call on a device sets up its status word: make one before capturing a graph")
+                status, host = _new_status(device)
+                torch.cuda.current_stream(device).synchronize()  # other streams may read the word from now on
+        else:
+            status, host = _new_status(device)
+        ws = _status_cache[device] = ForwardWorkspace(None, None, None, None, [], status, host)
+    return ws
 
 
 def _fail(ws, code: int, what: str):
@@ -224,3 +245,4 @@ def clear() -> None:
         _retire(ws)
     _fwd_cache.clear()
     _bwd_cache.clear()
+    _status_cache.clear()
