@@ -279,6 +279,37 @@ int rfa_scored_bwd_local(const void* q, const void* k, const void* v, const void
                          void* stream);
 
 /*
+ * K/V cache held in 4 bits.  A page holds 64 tokens of every head:
+ *   codes [n_pages, Hkv, 2 (K, V), 64, D / 2] bytes,  meta [n_pages, Hkv, 2, 64, D / 32, 2 (sc, min)] in dtype.
+ * A group of 32 channels holds u in 0..15 for each channel and stands for u * sc + min.  In a row of K the codes of channels
+ * [32 g + 8 c, + 8) are the 32-bit word c * D / 32 + g, in a row of V those of [32 g + 4 c, + 4) the 16-bit half word
+ * c * D / 32 + g, the first channel in the lowest bits.  D is 64, 96, 128, 192 or 256; codes and meta start on 16 bytes.
+ *  table      int32 [B, max_pages]: page of tokens [64 i, 64 i + 64) of a sequence; tokens on a page outside
+ *             [0, n_pages) do not exist
+ *
+ * rfa_kv4_append   writes tokens positions[b] + t, t < counts[b] (all T without counts), of k and v [B,T,Hkv,D] (strides of
+ *                  the first three dimensions in elements, multiples of 8): sc = (max - min) / 15 rounded to dtype,
+ *                  u = rint((x - min) / sc), 0 where sc is 0.  Tokens outside the table are left out.  No two tokens of a
+ *                  call may be the same row.
+ * rfa_kv4_gather   reads them back, rounded to dtype, into k and v [B,T,Hkv,D] (contiguous); zeros where there is no token.
+ * rfa_kv4_attn     attention of the last T tokens of each sequence (q [B,T,Hq,D] by strides) over its first lens[b] tokens,
+ *                  themselves included: token t sees keys up to lens[b] - T + t.  Scores as in rfa_score_args.  out
+ *                  [B,T,Hq,D], lse [B,Hq,T] or NULL; rows that see nothing get 0 and -inf.  Two launches.
+ *  scratch    rfa_kv4_scratch_elems floats (0: unsupported)
+ * positions, counts, lens: int32 [B], device memory; nothing is synchronised.  lens beyond the table end at it.
+ */
+size_t rfa_kv4_scratch_elems(int T, int Hq, int Hkv, int D);
+int rfa_kv4_append(const void* k, const void* v, const long long* k_strides, const long long* v_strides, void* codes,
+                   void* meta, int n_pages, const int* table, int max_pages, const int* positions, const int* counts, int B,
+                   int T, int Hkv, int D, int dtype, void* stream);
+int rfa_kv4_gather(void* k, void* v, const void* codes, const void* meta, int n_pages, const int* table, int max_pages,
+                   const int* positions, const int* counts, int B, int T, int Hkv, int D, int dtype, void* stream);
+int rfa_kv4_attn(const void* q, const long long* q_strides, const void* codes, const void* meta, int n_pages,
+                 const int* table, int max_pages, const int* lens, void* out, float* lse, float* scratch, int B, int T, int Hq,
+                 int Hkv, int D, int dtype, float softmax_scale, float softcap, const float* slopes, int slopes_per_batch,
+                 int* status, void* stream);
+
+/*
  * Packs K and V ([B, Skv, Hkv, D] each, `bytes_each` bytes) into one contiguous
  * [2, B, Skv, Hkv, D] transport buffer.  Replaces `kv_send[0].copy_(k);
  * kv_send[1].copy_(v)` (optimized_ring_flash_attn.py:836-838, 974-976).

@@ -53,6 +53,10 @@ SIGNATURES = {
     "rfa_scored_fwd_hop": (_i, [_vp] * 8 + [_i] * 6 + [_vp] + [_i] * 2 + [_vp] * 2),
     "rfa_scored_bwd_hop": (_i, [_vp] * 8 + [_i] * 6 + [_vp] * 4),
     "rfa_scored_bwd_local": (_i, [_vp] * 13 + [_i] * 6 + [_vp] * 4),
+    "rfa_kv4_scratch_elems": (_sz, [_i] * 4),
+    "rfa_kv4_append": (_i, [_vp] * 6 + [_i, _vp, _i] + [_vp] * 2 + [_i] * 5 + [_vp]),
+    "rfa_kv4_gather": (_i, [_vp] * 4 + [_i, _vp, _i] + [_vp] * 2 + [_i] * 5 + [_vp]),
+    "rfa_kv4_attn": (_i, [_vp] * 4 + [_i, _vp, _i] + [_vp] * 4 + [_i] * 6 + [_f] * 2 + [_vp, _i] + [_vp] * 2),
     "rfa_noalloc_scratch_bytes": (_sz, []),
     "rfa_bwd_hop_noalloc": (_i, [_vp] * 9 + [_i] * 7 + [_f] + [_i] * 2 + [_vp, _vp]),
     "rfa_dkdv_accumulate": (_i, [_vp, _vp, _vp, _sz, _vp]),
@@ -291,6 +295,45 @@ def scored_bwd_local(q, k, v, out, dout, lse, delta, lse2, dq_acc, dkdv, dq, dk,
             _ptr(dq), _ptr(dk), _ptr(dv), B, S, Hq, k.shape[2], D, DTYPE_CODES[q.dtype], ctypes.byref(args),
             _ptr(dq_order), _ptr(status), _stream(stream, q))
     _check(rc, "rfa_scored_bwd_local", kernels=3)
+
+
+def _strides(t: torch.Tensor):
+    return (ctypes.c_longlong * 3)(*t.stride()[:3])
+
+
+def kv4_append(k, v, codes, meta, table, positions, counts, stream=None) -> None:
+    B, T, Hkv, D = k.shape
+    with _on_device(k):
+        rc = load().rfa_kv4_append(_ptr(k), _ptr(v), _strides(k), _strides(v), _ptr(codes), _ptr(meta), codes.shape[0],
+                                   _ptr(table), table.shape[1], _ptr(positions), _ptr(counts), B, T, Hkv, D,
+                                   DTYPE_CODES[meta.dtype], _stream(stream, k))
+    _check(rc, "rfa_kv4_append")
+
+
+def kv4_gather(k, v, codes, meta, table, positions, counts, stream=None) -> None:
+    B, T, Hkv, D = k.shape
+    with _on_device(k):
+        rc = load().rfa_kv4_gather(_ptr(k), _ptr(v), _ptr(codes), _ptr(meta), codes.shape[0], _ptr(table), table.shape[1],
+                                   _ptr(positions), _ptr(counts), B, T, Hkv, D, DTYPE_CODES[meta.dtype], _stream(stream, k))
+    _check(rc, "rfa_kv4_gather")
+
+
+def kv4_scratch_elems(T: int, Hq: int, Hkv: int, D: int) -> int:
+    n = load().rfa_kv4_scratch_elems(T, Hq, Hkv, D)
+    if n == 0:
+        raise RuntimeError(f"unsupported sizes for attention over a 4-bit cache: T={T} Hq={Hq} Hkv={Hkv} D={D}")
+    return n
+
+
+def kv4_attn(q, codes, meta, table, lens, out, lse, scratch, softmax_scale: float, softcap: float, slopes, status,
+             stream=None) -> None:
+    B, T, Hq, D = q.shape
+    with _on_device(q):
+        rc = load().rfa_kv4_attn(_ptr(q), _strides(q), _ptr(codes), _ptr(meta), codes.shape[0], _ptr(table), table.shape[1],
+                                 _ptr(lens), _ptr(out), _ptr(lse), _ptr(scratch), B, T, Hq, codes.shape[1], D,
+                                 DTYPE_CODES[q.dtype], softmax_scale, softcap, _ptr(slopes),
+                                 int(slopes is not None and slopes.dim() == 2), _ptr(status), _stream(stream, q))
+    _check(rc, "rfa_kv4_attn", kernels=2)
 
 
 def bwd_hop_noalloc(q, k, v, dout, lse2, delta, dq, dkdv_prev, dkdv_out, softmax_scale: float,
