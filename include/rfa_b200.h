@@ -298,7 +298,7 @@ int rfa_scored_bwd_local(const void* q, const void* k, const void* v, const void
  *  scratch    rfa_kv4_scratch_elems floats (0: unsupported)
  * positions, counts, lens: int32 [B], device memory; nothing is synchronised.  lens beyond the table end at it.
  */
-size_t rfa_kv4_scratch_elems(int T, int Hq, int Hkv, int D);
+size_t rfa_kv4_scratch_elems(int B, int T, int Hq, int Hkv, int D);
 int rfa_kv4_append(const void* k, const void* v, const long long* k_strides, const long long* v_strides, void* codes,
                    void* meta, int n_pages, const int* table, int max_pages, const int* positions, const int* counts, int B,
                    int T, int Hkv, int D, int dtype, void* stream);

@@ -53,7 +53,7 @@ SIGNATURES = {
     "rfa_scored_fwd_hop": (_i, [_vp] * 8 + [_i] * 6 + [_vp] + [_i] * 2 + [_vp] * 2),
     "rfa_scored_bwd_hop": (_i, [_vp] * 8 + [_i] * 6 + [_vp] * 4),
     "rfa_scored_bwd_local": (_i, [_vp] * 13 + [_i] * 6 + [_vp] * 4),
-    "rfa_kv4_scratch_elems": (_sz, [_i] * 4),
+    "rfa_kv4_scratch_elems": (_sz, [_i] * 5),
     "rfa_kv4_append": (_i, [_vp] * 6 + [_i, _vp, _i] + [_vp] * 2 + [_i] * 5 + [_vp]),
     "rfa_kv4_gather": (_i, [_vp] * 4 + [_i, _vp, _i] + [_vp] * 2 + [_i] * 5 + [_vp]),
     "rfa_kv4_attn": (_i, [_vp] * 4 + [_i, _vp, _i] + [_vp] * 4 + [_i] * 6 + [_f] * 2 + [_vp, _i] + [_vp] * 2),
@@ -318,10 +318,10 @@ def kv4_gather(k, v, codes, meta, table, positions, counts, stream=None) -> None
     _check(rc, "rfa_kv4_gather")
 
 
-def kv4_scratch_elems(T: int, Hq: int, Hkv: int, D: int) -> int:
-    n = load().rfa_kv4_scratch_elems(T, Hq, Hkv, D)
+def kv4_scratch_elems(B: int, T: int, Hq: int, Hkv: int, D: int) -> int:
+    n = load().rfa_kv4_scratch_elems(B, T, Hq, Hkv, D)
     if n == 0:
-        raise RuntimeError(f"unsupported sizes for attention over a 4-bit cache: T={T} Hq={Hq} Hkv={Hkv} D={D}")
+        raise RuntimeError(f"unsupported sizes for attention over a 4-bit cache: B={B} T={T} Hq={Hq} Hkv={Hkv} D={D}")
     return n
 
 

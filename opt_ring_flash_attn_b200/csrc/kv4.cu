@@ -15,6 +15,7 @@ namespace rfa {
 constexpr int kPage = 64;    // tokens
 constexpr int kGroup = 32;   // channels
 constexpr int kSmCount = 148;
+constexpr int kMaxParts = kSmCount * 4;  // blocks of a launch at most
 
 // ----------------------------------------------------------------------------
 // Append and read-back: four lanes per group, eight channels each.  Bound by memory: 2 x 16 bytes in and 2 x 5 out per lane.
@@ -173,18 +174,26 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(T* __restrict__ k, T* _
 // ----------------------------------------------------------------------------
 // Attention of new tokens over the cache
 // ----------------------------------------------------------------------------
-// Bound by reading the cache (160 bytes per key and head at D = 128), so everything is arranged around a page once it is in
-// shared memory, and the pages of all sequences and heads are dealt out evenly: with units (b, kv head, tile of query rows)
-// laid end to end, block i takes pages [i q, (i + 1) q) of them all, whatever the lengths are.  A unit that several blocks
-// share is joined by a second kernel from at most two partial results per block.
+// What it cannot do without is one read of the cache (160 bytes per key and head at D = 128); what limits it beside that is
+// the logic unit, which works at half the rate of the others and has to take the codes apart.  So the arrangement is around
+// how few of its operations a code needs, and the pages of all sequences and heads are dealt out evenly: with units (b, kv
+// head, tile of query rows) laid end to end, block i takes pages [i q, (i + 1) q) of them all, whatever the lengths are.  A
+// unit that several blocks share is joined by a second kernel from at most two partial results per block.
 //
-// A block has a copying warp, which keeps kStages pages in flight, and four warps of 16 tokens each.  A warp computes, with
-// tokens as the 16 rows and query rows (tokens x heads of the group, 8 or 16) as the columns of m16n8k16 products,
-//   S[token][row] = sum over groups of sc_k * (u_k . q) + min_k * sum(q)        one accumulator per group
-//   O[channel][row] += u_v (P sc_v),   plus sum(P min_v) per group and row      sc_v folded into P
-// so the codes enter the tensor cores as they are: 4-bit codes become 16-bit floats by placing them in the mantissa of a power
-// of two (one logic operation per two codes).  K keeps that power in its products and takes it out through min; V subtracts
-// it, since there the sum runs over all tokens.  P sc_v is rounded to 16 bits like the P of the other kernels.
+// A block has two pairs of warps; a pair takes every other page of a run, a warp 32 of its 64 tokens, and the pair's first
+// warp keeps its pages coming through a ring of its own.  Tokens are the 16 rows, query rows (tokens x heads of the group, 8
+// or 16) the columns of the products:
+//   S[token][row] = sum over groups g of sc (u . q)  +  sum of min_g sum_g(q)
+//   O[channel][row] += u (P sc)  +  sum(P min) per group and row
+// A code in bits 0-3 or 4-7 of a half word read as fp16 is u 2^-24 or u 2^-20 (subnormal numbers, which the products take as
+// they are), so one logic operation takes two codes out and two of four need no shift.  (The same nibble as an e4m3 byte is
+// u 2^-9, one operation for four codes, but products of e4m3 are widened to fp16 on the same logic unit: 57 million
+// instructions instead of XX.)
+//   q enters as fp16, each row under a power of two and the channels of odd codes under 2^-4 of it: exact for fp16 and bf16.
+//   The minima meet the group sums of q, split in two 16-bit parts, in one more product with the meta words as they are.
+//   P sc is rounded to fp16 (11 bits, for bf16 caches too), under a power of two that keeps it in range.  For fp16 results
+//   u - 8 stands in for u, which halves what that rounding weighs (min + 8 sc makes up for it): relative error of fp16
+//   results 2.8e-4 instead of 4.8e-4, where rounding the result alone gives 2.1e-4.
 struct Kv4AttnParams {
   const void* q;
   const uint8_t* codes;
@@ -195,6 +204,7 @@ struct Kv4AttnParams {
   float* lse;
   float* part_o;   // [2 * blocks][rows][D]
   float* part_ml;  // [2 * blocks][rows][2]
+  int2* shared_by; // [B][units]: first and last block of the unit
   long long q_b, q_t, q_h;  // strides of q, in elements
   int B, T, Hq, Hkv, D;
   int n_pages, max_pages, units, blocks;  // units: (kv head, row tile) pairs of a sequence
@@ -209,32 +219,10 @@ __device__ __forceinline__ int kv4_len(const Kv4AttnParams& p, int b) {
 }
 __device__ __forceinline__ int pages_of(int len) { return (len + kPage - 1) / kPage; }
 
-// Pages of all units, by the whole block (its threads are a multiple of 32, `red` has a slot per warp).
-__device__ __forceinline__ long long kv4_total(const Kv4AttnParams& p, int before, long long* red, long long* sum_before) {
-  long long all = 0, prior = 0;
-  for (int b = threadIdx.x; b < p.B; b += blockDim.x) {
-    const int n = pages_of(kv4_len(p, b));
-    all += n;
-    if (b < before) prior += n;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-    prior += __shfl_xor_sync(0xffffffffu, prior, o);
-  }
-  if ((threadIdx.x & 31) == 0) {
-    red[2 * (threadIdx.x >> 5)] = all;
-    red[2 * (threadIdx.x >> 5) + 1] = prior;
-  }
-  __syncthreads();
-  all = prior = 0;
-  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) {
-    all += red[2 * w];
-    prior += red[2 * w + 1];
-  }
-  *sum_before = prior * p.units;
-  return all * p.units;
-}
+// The work of a unit in pages: its own, and kUnitCost for what comes with each unit (its queries, joining four warps' results,
+// writing them).  B 64, lengths to 8192: without it blocks with short sequences end at 126 us, the others at 79.
+constexpr int kUnitCost = 3;
+__device__ __forceinline__ int unit_work(int pages) { return pages > 0 ? pages + kUnitCost : 0; }
 
 // A position in the units laid end to end.
 struct Kv4Cursor {
@@ -253,60 +241,107 @@ struct Kv4Cursor {
       open(p);
     } while (pages == 0);
   }
+  // Pages of this unit for a block that has `work` left from here on, and what is left then.  A block that ends before the
+  // first page of a unit leaves the unit to the next one.
+  __device__ __forceinline__ int take(int& work, int& skip) const {
+    const int head = page == 0 ? kUnitCost - skip : 0;  // `skip`: of the unit's cost lies before the block
+    skip = 0;
+    const int n = max(0, min(work - head, pages - page));
+    work -= head + n;
+    return n;
+  }
 };
 
-// Page `at` of all; one warp, converged.
-__device__ __forceinline__ Kv4Cursor kv4_seek(const Kv4AttnParams& p, long long at) {
+// Work of all units, and the position `begin(total)` of it, with the part of the unit's cost that lies before the position;
+// one warp, converged.  Lengths of up to 32 sequences are read once.
+template <typename F>
+__device__ __forceinline__ Kv4Cursor kv4_seek(const Kv4AttnParams& p, F begin, int& total, int& skip) {
   const int lane = threadIdx.x & 31;
-  long long base = 0;
+  const int first = lane < p.B ? pages_of(kv4_len(p, lane)) : 0;
+  int sum = unit_work(first);
+  for (int b = lane + 32; b < p.B; b += 32) sum += unit_work(pages_of(kv4_len(p, b)));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  total = sum * p.units;
+  const int at = begin(total);
+  int base = 0;
   for (int b0 = 0;; b0 += 32) {
-    const int n = b0 + lane < p.B ? pages_of(kv4_len(p, b0 + lane)) : 0;
-    long long upto = static_cast<long long>(n) * p.units;
+    const int n = b0 == 0 ? first : b0 + lane < p.B ? pages_of(kv4_len(p, b0 + lane)) : 0;
+    int upto = unit_work(n) * p.units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += x;
     }
     const unsigned past = __ballot_sync(0xffffffffu, base + upto > at);
     if (past != 0 || b0 + 32 >= p.B) {
       const int l = past != 0 ? __ffs(past) - 1 : 31;
-      const long long before = l == 0 ? 0 : __shfl_sync(0xffffffffu, upto, l - 1 < 0 ? 0 : l - 1);
+      const int before = l == 0 ? 0 : __shfl_sync(0xffffffffu, upto, l - 1 < 0 ? 0 : l - 1);
       Kv4Cursor c;
       c.b = min(b0 + l, p.B - 1);
-      c.open(p);
-      const long long in = at - base - before;
-      c.u = c.pages > 0 ? static_cast<int>(in / c.pages) : 0;
-      c.page = c.pages > 0 ? static_cast<int>(in % c.pages) : 0;
+      c.len = kv4_len(p, c.b);
+      c.pages = pages_of(c.len);
+      const int in = at - base - before, each = max(unit_work(c.pages), 1);
+      c.u = in / each;
+      c.page = max(in % each - kUnitCost, 0);
+      skip = min(in % each, kUnitCost);
       return c;
     }
     base += __shfl_sync(0xffffffffu, upto, 31);
   }
 }
 
-// 4-bit codes at bits 0-3 and 16-19 of w, shifted there by `e` places of four, as a pair of 16-bit floats kBias + u.
-template <typename T, int e>
-__device__ __forceinline__ uint32_t codes_pair(uint32_t w) {
-  uint32_t r;
-  if constexpr (Pack2<T>::kIsBf16) {  // 128 + u: the code in the lowest bits of the 7-bit mantissa
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(e ? w >> (4 * e) : w), "r"(0x000f000fu), "r"(0x43004300u));
-  } else {  // 64 + u: at bits 4-7 of the 10-bit mantissa
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(e == 0 ? w << 4 : e == 1 ? w : w >> (4 * e - 4)), "r"(0x00f000f0u), "r"(0x54005400u));
+// Where the share of block i begins, in work of all units.  Every block that takes part has some: between the first and the
+// last block of a unit there is none without a part of it.
+__device__ __forceinline__ int block_start(const Kv4AttnParams& p, int total, int i) {
+  const int n = max(min(p.blocks, total), 1);
+  return static_cast<int>(static_cast<long long>(total) * min(i, n) / n);
+}
+
+// The pages that a pair of warps copies: every other one of each run.
+struct Kv4Fetch {
+  Kv4Cursor at;  // start of the run
+  int work, run, next, count;
+  // to the next page from `next` on, over the ends of runs; its number (read here, looked at one step later)
+  __device__ __forceinline__ int settle(const Kv4AttnParams& p, int first) {
+    while (next >= run) {
+      if (work <= 0) {
+        run = -1;
+        return -1;
+      }
+      at.next_unit(p);
+      int skip = 0;
+      run = at.take(work, skip);
+      next = first;
+    }
+    return __ldg(p.table + static_cast<size_t>(at.b) * p.max_pages + at.page + next);
   }
-  return r;
+};
+
+// The two halves of a meta word in fp32, by additions of mixed precision: a shift or a mask would go to the logic unit.
+template <typename T>
+__device__ __forceinline__ float wide_lo(uint32_t w) {
+  float y;
+  if constexpr (Pack2<T>::kIsBf16) asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tadd.rn.f32.bf16 %0, l, %2;\n\t}" : "=f"(y) : "r"(w), "f"(-0.f));
+  else asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tadd.rn.f32.f16 %0, l, %2;\n\t}" : "=f"(y) : "r"(w), "f"(-0.f));
+  return y;
 }
 template <typename T>
-__device__ __forceinline__ constexpr float codes_bias() { return Pack2<T>::kIsBf16 ? 128.f : 64.f; }
-template <typename T>
-__device__ __forceinline__ uint32_t minus_bias(uint32_t x) {
-  if constexpr (Pack2<T>::kIsBf16) {
-    const uint32_t b = 0x43004300u;
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  } else {
-    const uint32_t b = 0x54005400u;
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
+__device__ __forceinline__ float wide_hi(uint32_t w) {
+  float y;
+  if constexpr (Pack2<T>::kIsBf16) asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tadd.rn.f32.bf16 %0, h, %2;\n\t}" : "=f"(y) : "r"(w), "f"(-0.f));
+  else asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tadd.rn.f32.f16 %0, h, %2;\n\t}" : "=f"(y) : "r"(w), "f"(-0.f));
+  return y;
+}
+
+// Codes e and e + 4 of a word (one per half word) as fp16, (u - 8) or u times 2^-24 (e even) or 2^-20 (e odd).
+template <bool kCentred, int e>
+__device__ __forceinline__ uint32_t codes_fp16(uint32_t w) {
+  const uint32_t x = (e >= 2 ? w >> 8 : w) & (e % 2 ? 0x00f000f0u : 0x000f000fu);
+  if constexpr (!kCentred) return x;
+  const uint32_t eight = e % 2 ? 0x00800080u : 0x00080008u;
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&eight));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 template <typename T>
@@ -320,12 +355,12 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ float4 add4(const float4& a, const float4& b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // N 32-bit words from shared memory, as wide as their alignment (N words) allows.
 template <int N>
@@ -368,342 +403,467 @@ struct Kv4Cfg {
   static constexpr int kCodeBytes = 2 * kPage * kD / 2;
   static constexpr int kMetaBytes = 2 * kPage * NG * 4;
   static constexpr int kStageBytes = kCodeBytes + kMetaBytes;
-  static constexpr int kStages = NG <= 2 ? 6 : NG <= 4 ? 4 : 3;
-  static constexpr int kBlocksPerSm = NG * NT <= 4 ? 3 : 2;
-  static constexpr int kOffJoin = kStages * kStageBytes;           // [kRows][kD] fp32
-  static constexpr int kOffMl = kOffJoin + kRows * kD * 4;         // [4 warps][kRows][2]
+  static constexpr int kBlocksPerSm = NG * NT <= 4 ? 4 : NG * NT <= 6 ? 3 : 2;
+  static constexpr int kRing = NG <= 2 ? 4 : NG * NT <= 4 ? 2 : NG * NT <= 6 ? 2 : NG <= 4 ? 4 : 2;  // pages of a pair
+  static constexpr int kOffJoin = 2 * kRing * kStageBytes;         // [2 pairs][kRows][kD] fp32
+  static constexpr int kOffMl = kOffJoin + 2 * kRows * kD * 4;     // [4 warps][kRows][2]
   static constexpr int kSmemBytes = kOffMl + 4 * kRows * 2 * 4;
-  static_assert(kBlocksPerSm * (kSmemBytes + 1024) <= 228 * 1024, "shared memory over budget");
+  static_assert(kBlocksPerSm * (kSmemBytes + 1024 + 256) <= 228 * 1024, "shared memory over budget");
 };
 
 template <typename T, int NG, int NT>
-__global__ void __launch_bounds__(160, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_kernel(const Kv4AttnParams p) {
+__global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_kernel(const Kv4AttnParams p) {
   using Cfg = Kv4Cfg<NG, NT>;
-  constexpr int kStages = Cfg::kStages, kRows = Cfg::kRows, D = Cfg::kD;
+  constexpr int kRing = Cfg::kRing, kRows = Cfg::kRows, D = Cfg::kD;
+  constexpr bool kCentred = !Pack2<T>::kIsBf16;
+  constexpr int kQuads = (NG + 3) / 4;
+  constexpr float q_down = 1.f / 16777216.f;  // codes are u 2^-24
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t bar_full[kStages], bar_empty[kStages];
-  __shared__ int page_ok[kStages];
-  __shared__ long long red[2 * 5];
+  __shared__ uint64_t bar_full[2][kRing], bar_empty[2][kRing];
+  __shared__ int page_ok[2][kRing];
+  __shared__ Kv4Fetch fetcher[2];
   __shared__ int abort_flag, skip_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pair = warp >> 1, side = warp & 1;
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&bar_full[i], 1);
-      mbar_init(&bar_empty[i], 4);
+    for (int i = 0; i < 2 * kRing; ++i) {
+      mbar_init(&bar_full[0][i], 1);
+      mbar_init(&bar_empty[0][i], 1);
     }
     mbar_fence_init();
   }
   pdl_wait();
   pdl_trigger();  // the joining kernel waits for this one's results itself
   if (threadIdx.x == 0) skip_flag = *reinterpret_cast<volatile int*>(p.status);
-  long long unused;
-  const long long total = kv4_total(p, 0, red, &unused);  // a block barrier inside: the barriers are ready behind it
-  if (skip_flag != 0) return;
-  const long long quota = (total + p.blocks - 1) / p.blocks;
-  const long long begin = min(quota * blockIdx.x, total), end = min(begin + quota, total);
-  if (begin >= end) return;
   volatile int* abort_p = &abort_flag;
-  Kv4Cursor at = kv4_seek(p, begin);
-  int left = static_cast<int>(end - begin);
+  int total, skip;
+  Kv4Cursor at = kv4_seek(p, [&](int all) { return block_start(p, all, blockIdx.x); }, total, skip);
+  int work = block_start(p, total, blockIdx.x + 1) - block_start(p, total, blockIdx.x);
+  __syncthreads();  // the barriers are ready
+  if (skip_flag != 0 || work <= 0) return;
   const int n_row_tiles = p.units / p.Hkv;
+  uint8_t* const ring = smem + pair * (kRing * Cfg::kStageBytes);
 
-  if (warp == 4) {
-    // =========================== copying warp ===========================
-    int n = 0;
-    bool ok = true;
-    while (left > 0 && ok) {
-      const int run = min(left, at.pages - at.page);
-      const int head = at.u / n_row_tiles;
-      for (int i0 = 0; i0 < run && ok; i0 += 32) {
-        const int mine = i0 + lane < run ? __ldg(p.table + static_cast<size_t>(at.b) * p.max_pages + at.page + i0 + lane) : -1;
-        for (int i = 0; i < min(32, run - i0); ++i, ++n) {
-          const int page = __shfl_sync(0xffffffffu, mine, i);
-          const int st = n % kStages;
-          if (lane == 0) {
-            ok = mbar_wait(&bar_empty[st], ((n / kStages) & 1) ^ 1, abort_p);
-            if (ok) {
-              uint8_t* dst = smem + st * Cfg::kStageBytes;
-              const bool good = page >= 0 && page < p.n_pages;
-              page_ok[st] = good;
-              if (good) {
-                const size_t slab = static_cast<size_t>(page) * p.Hkv + head;
-                mbar_expect_tx(&bar_full[st], Cfg::kStageBytes);
-                bulk_load_1d(smem_u32(dst), p.codes + slab * Cfg::kCodeBytes, Cfg::kCodeBytes, &bar_full[st]);
-                bulk_load_1d(smem_u32(dst + Cfg::kCodeBytes), static_cast<const uint8_t*>(p.meta) + slab * Cfg::kMetaBytes,
-                             Cfg::kMetaBytes, &bar_full[st]);
-              } else {
-                mbar_arrive(&bar_full[st]);  // a page outside the pool: its tokens are not there
-              }
-            }
-          }
-          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-          if (!ok) break;
-        }
-      }
-      left -= run;
-      at.next_unit(p);
+  // ---- the copies of a pair: lane 0 of its first warp walks the same pages, kRing ahead ----
+  // Its state lives in shared memory (one lane needs it), and the number of the next page is read one step early (in a register:
+  // a store of it would wait for the load).
+  int next_page = -1;
+  bool ok = true;  // after a wait that ran out nothing is computed, but every barrier of the block is still met
+  auto fetch = [&]() {  // the next page of the pair, if there is one, into the slot that has its turn
+    Kv4Fetch& f = fetcher[pair];
+    if (f.run < 0) return true;
+    const int slot = f.count % kRing;
+    if (f.count >= kRing && !mbar_wait(&bar_empty[pair][slot], (f.count / kRing - 1) & 1, abort_p)) return false;
+    const bool good = next_page >= 0 && next_page < p.n_pages;
+    page_ok[pair][slot] = good;
+    if (good) {
+      const size_t slab = static_cast<size_t>(next_page) * p.Hkv + f.at.u / n_row_tiles;
+      uint8_t* dst = ring + slot * Cfg::kStageBytes;
+      mbar_expect_tx(&bar_full[pair][slot], Cfg::kStageBytes);
+      bulk_load_1d(smem_u32(dst), p.codes + slab * Cfg::kCodeBytes, Cfg::kCodeBytes, &bar_full[pair][slot]);
+      bulk_load_1d(smem_u32(dst + Cfg::kCodeBytes), static_cast<const uint8_t*>(p.meta) + slab * Cfg::kMetaBytes,
+                   Cfg::kMetaBytes, &bar_full[pair][slot]);
+    } else {
+      mbar_arrive(&bar_full[pair][slot]);  // a page outside the pool: its tokens are not there
     }
-  } else {
-    // =========================== the warps that compute ===========================
-    const int r = lane >> 2, c = lane & 3;  // S row / O row group, and column pair
-    const int G = p.Hq / p.Hkv;
-    const float bias = codes_bias<T>();
-    int n = 0;
-    bool ok = true;  // after a wait that ran out nothing is computed, but every barrier of the block is still met
-    while (left > 0) {
-      const int run = min(left, at.pages - at.page);
-      const int head = at.u / n_row_tiles, row0 = at.u % n_row_tiles * kRows;
-      const int n_rows = p.T * G;
-      // Query rows as the B operand: lane holds channels [32 g + 8 c, + 8) of row r of each column tile, and the group sums
-      uint32_t qf[NT][NG][4];
-      float qsum[NT][NG][2], slope[NT][2];
-      int lim[NT][2];  // last key that the row sees
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int row = row0 + nt * 8 + r;
-        const T* src = static_cast<const T*>(p.q) + at.b * p.q_b + (row / G) * p.q_t + (head * G + row % G) * p.q_h + c * 8;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (row < n_rows) x = __ldg(reinterpret_cast<const uint4*>(src + g * kGroup));
-          // pairs (0,4) (1,5) (2,6) (3,7): the order in which shifts bring the codes of a word out
-          qf[nt][g][0] = __byte_perm(x.x, x.z, 0x5410);
-          qf[nt][g][1] = __byte_perm(x.x, x.z, 0x7632);
-          qf[nt][g][2] = __byte_perm(x.y, x.w, 0x5410);
-          qf[nt][g][3] = __byte_perm(x.y, x.w, 0x7632);
-          float s = (Kv4Type<T>::lo(x.x) + Kv4Type<T>::hi(x.x)) + (Kv4Type<T>::lo(x.y) + Kv4Type<T>::hi(x.y)) +
-                    (Kv4Type<T>::lo(x.z) + Kv4Type<T>::hi(x.z)) + (Kv4Type<T>::lo(x.w) + Kv4Type<T>::hi(x.w));
-          s += __shfl_xor_sync(0xffffffffu, s, 1);
-          s += __shfl_xor_sync(0xffffffffu, s, 2);
-          qsum[nt][g][0] = __shfl_sync(0xffffffffu, s, (2 * c) * 4);  // of the columns 2 c and 2 c + 1 that this lane has in S
-          qsum[nt][g][1] = __shfl_sync(0xffffffffu, s, (2 * c + 1) * 4);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int col = row0 + nt * 8 + 2 * c + i;
-          lim[nt][i] = col < n_rows ? at.len - p.T + col / G : -1;
-          slope[nt][i] = 0.f;
-          if (p.slopes && col < n_rows)
-            slope[nt][i] = __ldg(p.slopes + (p.slopes_per_batch ? static_cast<size_t>(at.b) * p.Hq : 0) + head * G + col % G) * kLog2e;
-        }
-      }
-      float o[NT][NG][2][4], corr[NT][NG][2], m[NT][2], l[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[nt][g][0][i] = o[nt][g][1][i] = 0.f;
-          corr[nt][g][0] = corr[nt][g][1] = 0.f;
-        }
-        m[nt][0] = m[nt][1] = kNoKey;
-        l[nt][0] = l[nt][1] = 0.f;
-      }
+    ++f.count;
+    f.next += 2;
+    next_page = f.settle(p, pair);
+    return true;
+  };
+  if (side == 0 && lane == 0) {
+    Kv4Fetch& f = fetcher[pair];
+    int f_skip = skip;
+    f.at = at;
+    f.work = work;
+    f.run = at.take(f.work, f_skip);
+    f.next = pair;
+    f.count = 0;
+    next_page = f.settle(p, pair);
+    for (int i = 0; i < kRing; ++i) fetch();  // no waits yet
+  }
 
-      for (int i = 0; i < run; ++i, ++n) {
-        const int st = n % kStages;
-        ok = ok && mbar_wait_warp(&bar_full[st], (n / kStages) & 1, abort_p);
-        if (!ok) continue;
-        const uint8_t* stage = smem + st * Cfg::kStageBytes;
-        const int pos0 = (at.page + i) * kPage + warp * 16;  // of the warp's first token
-        const int there = page_ok[st] ? at.len - pos0 : 0;   // tokens of the warp that exist
-        if (there > 0) {
-          const bool tail = pos0 + 15 > at.len - p.T;  // some row does not see all of them
-          const uint8_t* kc = stage + (warp * 16 + r) * (D / 2) + c * NG * 4;
-          const uint8_t* km = stage + Cfg::kCodeBytes + (warp * 16 + r) * (NG * 4);
-          // ---- S ----
-          float s[NT][4];
+  const int r = lane >> 2, c = lane & 3;  // S row / O row group, and column pair
+  // S row r is token rt of each 8: V's loads then take tokens 0, 3, 4, 7 at a time, which lie in different banks by twos.
+  const int rt = r ^ ((r >> 1) & 1);
+  const int G = p.Hq / p.Hkv;
+  const int n_rows = p.T * G;
+  int n = 0;  // pages of the pair so far
+  while (work > 0) {
+    const int run = at.take(work, skip);
+    if (run == 0) {  // the share ends before the first page of this unit, or begins behind the last of the one before
+      at.next_unit(p);
+      continue;
+    }
+    const int head = at.u / n_row_tiles, row0 = at.u % n_row_tiles * kRows;
+    // Query rows as the B operand: this lane holds channels [32 g + 8 c, + 8) of row r of each column tile.
+    uint32_t qf[NT][NG][4], qs[NT][kQuads][2];
+    float zs[NT][2], slope[NT][2];
+    int lim[NT][2];  // last key that the row sees
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = row0 + nt * 8 + r;
+      const T* src = static_cast<const T*>(p.q) + at.b * p.q_b + (row / G) * p.q_t + (head * G + row % G) * p.q_h + c * 8;
+      uint4 x[NG];
+      float top = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        x[g] = make_uint4(0, 0, 0, 0);
+        if (row < n_rows) x[g] = __ldg(reinterpret_cast<const uint4*>(src + g * kGroup));
+        const uint32_t w[4] = {x[g].x, x[g].y, x[g].z, x[g].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max3_nan(top, fabsf(Kv4Type<T>::lo(w[i])), fabsf(Kv4Type<T>::hi(w[i])));
+      }
+      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^e with which the row's largest element comes to [2^12, 2^13): what lies 2^22 below it keeps its bits
+      const int ex = static_cast<int>(__float_as_uint(top) >> 23);  // 255: no number
+      const int e = ex == 255 ? 0 : min(139 - ex, 126);
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23), up_odd = 0.0625f * up;
+#pragma unroll
+      for (int k = 0; k < kQuads; ++k) qs[nt][k][0] = qs[nt][k][1] = 0;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float v0 = Kv4Type<T>::lo(x[g].x) * up, v1 = Kv4Type<T>::hi(x[g].x) * up_odd;
+        const float v2 = Kv4Type<T>::lo(x[g].y) * up, v3 = Kv4Type<T>::hi(x[g].y) * up_odd;
+        const float v4 = Kv4Type<T>::lo(x[g].z) * up, v5 = Kv4Type<T>::hi(x[g].z) * up_odd;
+        const float v6 = Kv4Type<T>::lo(x[g].w) * up, v7 = Kv4Type<T>::hi(x[g].w) * up_odd;
+        // pairs (0,4) (1,5) (2,6) (3,7): the order in which the codes of a word come out
+        qf[nt][g][0] = Pack2<__half>::pack(v0, v4);
+        qf[nt][g][1] = Pack2<__half>::pack(v1, v5);
+        qf[nt][g][2] = Pack2<__half>::pack(v2, v6);
+        qf[nt][g][3] = Pack2<__half>::pack(v3, v7);
+        float sum = fmaf(16.f, (v1 + v3) + (v5 + v7), (v0 + v2) + (v4 + v6));
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (g % 4 == c) {  // beside the minimum (upper half of a meta word) the sum of q, in two parts
+          sum *= q_down;
+          const uint16_t hi = Kv4Type<T>::bits(sum);
+          qs[nt][g / 4][0] = static_cast<uint32_t>(hi) << 16;
+          qs[nt][g / 4][1] = static_cast<uint32_t>(Kv4Type<T>::bits(sum - Kv4Type<T>::value(hi))) << 16;
+        }
+      }
+      // what brings the row's scores back, and a row that holds no number makes all of its scores none
+      const float back = ex == 255 ? __uint_as_float(0x7fc00000u) : 1.f / (up * q_down);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int col = row0 + nt * 8 + 2 * c + i;
+        zs[nt][i] = __shfl_sync(0xffffffffu, back, (2 * c + i) * 4) * (p.cap_log2 > 0.f ? p.cap_in : p.scale_log2);
+        lim[nt][i] = col < n_rows ? at.len - p.T + col / G : -1;
+        slope[nt][i] = 0.f;
+        if (p.slopes && col < n_rows)
+          slope[nt][i] = __ldg(p.slopes + (p.slopes_per_batch ? static_cast<size_t>(at.b) * p.Hq : 0) + head * G + col % G) * kLog2e;
+      }
+    }
+    float o[NT][NG][2][4], corr[NT][NG][2], m[NT][2], l[NT][2];
+    float v_down = 1.f, v_limit = 0.f;  // power of two on the scales of V, and the largest scale it is good for
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nt][g][0][i] = o[nt][g][1][i] = 0.f;
+        corr[nt][g][0] = corr[nt][g][1] = 0.f;
+      }
+      m[nt][0] = m[nt][1] = kNoKey;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+
+    for (int i = pair; i < run; i += 2, ++n) {
+      const int slot = n % kRing;
+      if (side == 0 && n > 0) {  // refill the slot before this one: the partner is done with it, or nearly
+        if (lane == 0 && ok) ok = fetch();
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      }
+      ok = ok && mbar_wait_warp(&bar_full[pair][slot], (n / kRing) & 1, abort_p);
+      if (!ok) continue;
+      const uint8_t* stage = ring + slot * Cfg::kStageBytes;
+      const int pos0 = (at.page + i) * kPage + side * 32;         // of the warp's first token
+      const int there = page_ok[pair][slot] ? at.len - pos0 : 0;  // tokens of the warp that exist
+      if (there > 0) {
+        const uint8_t* kc = stage + (side * 32 + rt) * (D / 2) + c * NG * 4;
+        const uint8_t* km = stage + Cfg::kCodeBytes + (side * 32 + rt) * (NG * 4);
+        // ---- S, tokens pos0 + 16 j + r and + 8 ----
+        float s[2][NT][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t w0[NG], w1[NG], e0[NG], e1[NG];
+          lds_words<NG>(w0, kc + j * 16 * (D / 2));
+          lds_words<NG>(w1, kc + (j * 16 + 8) * (D / 2));
+          lds_words<NG>(e0, km + j * 16 * (NG * 4));
+          lds_words<NG>(e1, km + (j * 16 + 8) * (NG * 4));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) s[nt][x] = 0.f;
-          uint32_t w0[NG], w1[NG], e0[NG], e1[NG];
-          lds_words<NG>(w0, kc);
-          lds_words<NG>(w1, kc + 8 * (D / 2));
-          lds_words<NG>(e0, km);
-          lds_words<NG>(e1, km + 8 * (NG * 4));
+            for (int x = 0; x < 4; ++x) s[j][nt][x] = 0.f;
+#pragma unroll
+          for (int k = 0; k < kQuads; ++k) {
+            const bool any = k * 4 + c < NG;
+            const uint32_t a = any ? *reinterpret_cast<const uint32_t*>(km + j * 16 * (NG * 4) + (k * 4 + c) * 4) : 0;
+            const uint32_t b = any ? *reinterpret_cast<const uint32_t*>(km + (j * 16 + 8) * (NG * 4) + (k * 4 + c) * 4) : 0;
+            const uint32_t mw[4] = {a, b, a, b};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<T>(s[j][nt], mw, qs[nt][k][0], qs[nt][k][1]);
+          }
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            const uint32_t a0[4] = {codes_pair<T, 0>(w0[g]), codes_pair<T, 0>(w1[g]), codes_pair<T, 1>(w0[g]), codes_pair<T, 1>(w1[g])};
-            const uint32_t a1[4] = {codes_pair<T, 2>(w0[g]), codes_pair<T, 2>(w1[g]), codes_pair<T, 3>(w0[g]), codes_pair<T, 3>(w1[g])};
-            const float sc0 = Kv4Type<T>::lo(e0[g]), mn0 = fmaf(-bias, sc0, Kv4Type<T>::hi(e0[g]));
-            const float sc1 = Kv4Type<T>::lo(e1[g]), mn1 = fmaf(-bias, sc1, Kv4Type<T>::hi(e1[g]));
+            const uint32_t a0[4] = {codes_fp16<false, 0>(w0[g]), codes_fp16<false, 0>(w1[g]), codes_fp16<false, 1>(w0[g]), codes_fp16<false, 1>(w1[g])};
+            const uint32_t a1[4] = {codes_fp16<false, 2>(w0[g]), codes_fp16<false, 2>(w1[g]), codes_fp16<false, 3>(w0[g]), codes_fp16<false, 3>(w1[g])};
+            const float sc0 = Kv4Type<T>::lo(e0[g]), sc1 = Kv4Type<T>::lo(e1[g]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               float acc[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816<T>(acc, a0, qf[nt][g][0], qf[nt][g][1]);
-              mma16816<T>(acc, a1, qf[nt][g][2], qf[nt][g][3]);
-              s[nt][0] = fmaf(acc[0], sc0, fmaf(mn0, qsum[nt][g][0], s[nt][0]));
-              s[nt][1] = fmaf(acc[1], sc0, fmaf(mn0, qsum[nt][g][1], s[nt][1]));
-              s[nt][2] = fmaf(acc[2], sc1, fmaf(mn1, qsum[nt][g][0], s[nt][2]));
-              s[nt][3] = fmaf(acc[3], sc1, fmaf(mn1, qsum[nt][g][1], s[nt][3]));
+              mma16816<__half>(acc, a0, qf[nt][g][0], qf[nt][g][1]);
+              mma16816<__half>(acc, a1, qf[nt][g][2], qf[nt][g][3]);
+              s[j][nt][0] = fmaf(acc[0], sc0, s[j][nt][0]);
+              s[j][nt][1] = fmaf(acc[1], sc0, s[j][nt][1]);
+              s[j][nt][2] = fmaf(acc[2], sc1, s[j][nt][2]);
+              s[j][nt][3] = fmaf(acc[3], sc1, s[j][nt][3]);
             }
           }
-          // ---- scores in log2 units, masks, running maximum ----
-          bool grow = false;
+        }
+        // ---- scores in log2 units, masks ----
+        if (p.cap_log2 > 0.f) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              float z = s[nt][x];
-              const int ahead = lim[nt][x & 1] - (pos0 + r + (x < 2 ? 0 : 8));  // of the row over this key
-              if (p.cap_log2 > 0.f) z = fmaf(-2.f * p.cap_log2, fast_rcp(fast_exp2(z * p.cap_in) + 1.f), p.cap_log2);
-              else z *= p.scale_log2;
-              if (p.slopes) z = fmaf(-slope[nt][x & 1], static_cast<float>(ahead), z);
-              if (tail && ahead < 0) z = -INFINITY;
-              s[nt][x] = z;
-              // the maximum follows when a score is more than 2^2 above it (P sc_v then stays below the largest fp16), or
-              // is no number
-              grow = grow || !(z - m[nt][x & 1] <= 2.f);
-            }
-          if (__any_sync(0xffffffffu, grow)) {
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                float top = max3_nan(m[nt][x], s[nt][x], s[nt][x + 2]);
+              for (int x = 0; x < 4; ++x)
+                s[j][nt][x] = fmaf(-2.f * p.cap_log2, fast_rcp(fast_exp2(s[j][nt][x] * zs[nt][x & 1]) + 1.f), p.cap_log2);
+        } else {
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
-                const float alpha = fast_exp2(m[nt][x] - top);
-                m[nt][x] = top;
-                l[nt][x] *= alpha;
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                  corr[nt][g][x] *= alpha;
-                  o[nt][g][0][x] *= alpha;
-                  o[nt][g][0][x + 2] *= alpha;
-                  o[nt][g][1][x] *= alpha;
-                  o[nt][g][1][x + 2] *= alpha;
-                }
-              }
-          }
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              s[nt][x] = fast_exp2(s[nt][x] - m[nt][x & 1]);
-              l[nt][x & 1] += s[nt][x];
-            }
-          // ---- O ----
-          const uint8_t* vc = stage + kPage * (D / 2) + (warp * 16 + 2 * c) * (D / 2) + r * NG * 2;
-          lds_words<NG>(e0, km + kPage * (NG * 4));
-          lds_words<NG>(e1, km + (kPage + 8) * (NG * 4));
-          if (r >= there) {  // tokens behind the last: their scales may be anything
-#pragma unroll
-            for (int g = 0; g < NG; ++g) e0[g] = 0;
-          }
-          if (r + 8 >= there) {
-#pragma unroll
-            for (int g = 0; g < NG; ++g) e1[g] = 0;
-          }
-          uint32_t t0[(NG + 1) / 2], t1[(NG + 1) / 2], t8[(NG + 1) / 2], t9[(NG + 1) / 2];
-          lds_halves<NG>(t0, vc);
-          lds_halves<NG>(t1, vc + D / 2);
-          lds_halves<NG>(t8, vc + 8 * (D / 2));
-          lds_halves<NG>(t9, vc + 9 * (D / 2));
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const uint32_t lo = __byte_perm(t0[g / 2], t1[g / 2], g % 2 ? 0x7632 : 0x5410);
-            const uint32_t hi = __byte_perm(t8[g / 2], t9[g / 2], g % 2 ? 0x7632 : 0x5410);
-            const uint32_t a0[4] = {minus_bias<T>(codes_pair<T, 0>(lo)), minus_bias<T>(codes_pair<T, 1>(lo)),
-                                    minus_bias<T>(codes_pair<T, 0>(hi)), minus_bias<T>(codes_pair<T, 1>(hi))};
-            const uint32_t a1[4] = {minus_bias<T>(codes_pair<T, 2>(lo)), minus_bias<T>(codes_pair<T, 3>(lo)),
-                                    minus_bias<T>(codes_pair<T, 2>(hi)), minus_bias<T>(codes_pair<T, 3>(hi))};
-            const float sc0 = Kv4Type<T>::lo(e0[g]), mn0 = Kv4Type<T>::hi(e0[g]);
-            const float sc1 = Kv4Type<T>::lo(e1[g]), mn1 = Kv4Type<T>::hi(e1[g]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const uint32_t b0 = transpose8x8(Pack2<T>::pack(s[nt][0] * sc0, s[nt][1] * sc0));
-              const uint32_t b1 = transpose8x8(Pack2<T>::pack(s[nt][2] * sc1, s[nt][3] * sc1));
-              corr[nt][g][0] = fmaf(s[nt][0], mn0, fmaf(s[nt][2], mn1, corr[nt][g][0]));
-              corr[nt][g][1] = fmaf(s[nt][1], mn0, fmaf(s[nt][3], mn1, corr[nt][g][1]));
-              mma16816<T>(o[nt][g][0], a0, b0, b1);
-              mma16816<T>(o[nt][g][1], a1, b0, b1);
-            }
-          }
+              for (int x = 0; x < 4; ++x) s[j][nt][x] *= zs[nt][x & 1];
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_empty[st]);
-      }
-
-      // ---- the four warps' results of this run into one ----
-      float* join = reinterpret_cast<float*>(smem + Cfg::kOffJoin);
-      float* ml = reinterpret_cast<float*>(smem + Cfg::kOffMl);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) {
-            l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], d);
-#pragma unroll
-            for (int g = 0; g < NG; ++g) corr[nt][g][x] += __shfl_xor_sync(0xffffffffu, corr[nt][g][x], d);
-          }
-          if (r == 0) {
-            ml[(warp * kRows + nt * 8 + 2 * c + x) * 2] = m[nt][x];
-            ml[(warp * kRows + nt * 8 + 2 * c + x) * 2 + 1] = l[nt][x];
-          }
-        }
-      consumers_sync();
-      float top[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          top[nt][x] = kNoKey;
-          for (int w = 0; w < 4; ++w) top[nt][x] = max_nan(top[nt][x], ml[(w * kRows + nt * 8 + 2 * c + x) * 2]);
-        }
-      for (int w = 0; w < 4; ++w) {  // in the order of the warps: the same sum every time
-        if (w == warp) {
+        if (p.slopes) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const float f = fast_exp2(m[nt][x] - top[nt][x]);
+              const float ahead = static_cast<float>(lim[nt][x] - (pos0 + rt));  // of the row over its first key here
 #pragma unroll
-              for (int g = 0; g < NG; ++g) {  // channels 32 g + 4 r + (0..3)
-                float4* dst = reinterpret_cast<float4*>(join + (nt * 8 + 2 * c + x) * D + g * kGroup + 4 * r);
-                const float4 old = w == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *dst;
-                *dst = make_float4(fmaf(o[nt][g][0][x] + corr[nt][g][x], f, old.x), fmaf(o[nt][g][0][x + 2] + corr[nt][g][x], f, old.y),
-                                   fmaf(o[nt][g][1][x] + corr[nt][g][x], f, old.z), fmaf(o[nt][g][1][x + 2] + corr[nt][g][x], f, old.w));
+              for (int j = 0; j < 2; ++j) {
+                s[j][nt][x] = fmaf(-slope[nt][x], ahead - 16.f * j, s[j][nt][x]);
+                s[j][nt][x + 2] = fmaf(-slope[nt][x], ahead - (16.f * j + 8.f), s[j][nt][x + 2]);
               }
             }
         }
-        consumers_sync();
-      }
-      const bool whole = at.page == 0 && run == at.pages;
-      const int slot = 2 * blockIdx.x + (at.page > 0 ? 0 : 1);
-      for (int i = threadIdx.x; i < kRows * D / 8; i += 128) {
-        const int row = i / (D / 8), ch = i % (D / 8) * 8, rg = row0 + row;
-        if (rg >= n_rows) continue;
-        float mm = kNoKey, ll = 0.f;
-        for (int w = 0; w < 4; ++w) mm = max_nan(mm, ml[(w * kRows + row) * 2]);
-        for (int w = 0; w < 4; ++w) ll += ml[(w * kRows + row) * 2 + 1] * fast_exp2(ml[(w * kRows + row) * 2] - mm);
-        const float4 x = *reinterpret_cast<const float4*>(join + row * D + ch);
-        const float4 y = *reinterpret_cast<const float4*>(join + row * D + ch + 4);
-        if (whole) {
-          const int t = rg / G, h = head * G + rg % G;
-          const float inv = ll == 0.f ? 0.f : 1.f / ll;
-          T* dst = static_cast<T*>(p.out) + ((static_cast<size_t>(at.b) * p.T + t) * p.Hq + h) * D + ch;
-          *reinterpret_cast<uint4*>(dst) = make_uint4(Pack2<T>::pack(x.x * inv, x.y * inv), Pack2<T>::pack(x.z * inv, x.w * inv),
-                                                      Pack2<T>::pack(y.x * inv, y.y * inv), Pack2<T>::pack(y.z * inv, y.w * inv));
-          if (p.lse && ch == 0)
-            p.lse[(static_cast<size_t>(at.b) * p.Hq + h) * p.T + t] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) / kLog2e;
-        } else {
-          float* dst = p.part_o + (static_cast<size_t>(slot) * kRows + row) * D + ch;
-          *reinterpret_cast<float4*>(dst) = x;
-          *reinterpret_cast<float4*>(dst + 4) = y;
-          if (ch == 0) *reinterpret_cast<float2*>(p.part_ml + (static_cast<size_t>(slot) * kRows + row) * 2) = make_float2(mm, ll);
+        if (pos0 + 31 > at.len - p.T) {  // some row does not see all of them
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                if (pos0 + j * 16 + rt + (x < 2 ? 0 : 8) > lim[nt][x & 1]) s[j][nt][x] = -INFINITY;
+        }
+        // ---- running maximum: it follows when a score is more than 2^2 above it, or is no number ----
+        bool grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float hi = max_nan(max3_nan(s[0][nt][x], s[0][nt][x + 2], s[1][nt][x]), s[1][nt][x + 2]);
+            grow = grow || !(hi - m[nt][x] <= 2.f);
+          }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              float top = max3_nan(m[nt][x], max_nan(s[0][nt][x], s[0][nt][x + 2]), max_nan(s[1][nt][x], s[1][nt][x + 2]));
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+              const float alpha = fast_exp2(m[nt][x] - top);
+              m[nt][x] = top;
+              l[nt][x] *= alpha;
+#pragma unroll
+              for (int g = 0; g < NG; ++g) {
+                corr[nt][g][x] *= alpha;
+                o[nt][g][0][x] *= alpha;
+                o[nt][g][0][x + 2] *= alpha;
+                o[nt][g][1][x] *= alpha;
+                o[nt][g][1][x + 2] *= alpha;
+              }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              s[j][nt][x] = fast_exp2(s[j][nt][x] - m[nt][x & 1]);
+              l[nt][x & 1] += s[j][nt][x];
+            }
+        // ---- O ----
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint8_t* vc = stage + kPage * (D / 2) + (side * 32 + j * 16 + 2 * c + (c & 1)) * (D / 2) + r * NG * 2;
+          const int v_next = (c & 1) ? -(D / 2) : D / 2;  // to the odd one of the two tokens
+          const uint8_t* vm = km + (kPage + j * 16) * (NG * 4);
+          uint32_t e0[NG], e1[NG];
+          lds_words<NG>(e0, vm);
+          lds_words<NG>(e1, vm + 8 * (NG * 4));
+          if (there < 32) {  // tokens behind the last: their scales may be anything
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              if (j * 16 + rt >= there) e0[g] = 0;
+              if (j * 16 + rt + 8 >= there) e1[g] = 0;
+            }
+          }
+          float sc0[NG], sc1[NG], most = 0.f;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            sc0[g] = Kv4Type<T>::lo(e0[g]);
+            sc1[g] = Kv4Type<T>::lo(e1[g]);
+            most = max3_nan(most, sc0[g], sc1[g]);
+          }
+          if (__any_sync(0xffffffffu, !(most <= v_limit))) {
+            // the first scales, or 2^8 above those the power was chosen for: it is chosen again, the largest comes to [1, 2)
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
+            const int ex = min(max(static_cast<int>(__float_as_uint(most) >> 23), 10), 245);
+            const float down = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
+            const float f = down / v_down;
+            v_down = down;
+            v_limit = __uint_as_float(static_cast<uint32_t>(min(ex + 8, 254)) << 23);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  o[nt][g][0][x] *= f;
+                  o[nt][g][1][x] *= f;
+                }
+          }
+          float pd[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) pd[nt][x] = s[j][nt][x] * v_down;
+          uint32_t t0[(NG + 1) / 2], t1[(NG + 1) / 2], t8[(NG + 1) / 2], t9[(NG + 1) / 2];
+          lds_halves<NG>(t0, vc);
+          lds_halves<NG>(t1, vc + v_next);
+          lds_halves<NG>(t8, vc + 8 * (D / 2));
+          lds_halves<NG>(t9, vc + 8 * (D / 2) + v_next);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const uint32_t lo = __byte_perm(t0[g / 2], t1[g / 2], g % 2 ? 0x7632 : 0x5410);
+            const uint32_t hi = __byte_perm(t8[g / 2], t9[g / 2], g % 2 ? 0x7632 : 0x5410);
+            const uint32_t a0[4] = {codes_fp16<kCentred, 0>(lo), codes_fp16<kCentred, 1>(lo), codes_fp16<kCentred, 0>(hi), codes_fp16<kCentred, 1>(hi)};
+            const uint32_t a1[4] = {codes_fp16<kCentred, 2>(lo), codes_fp16<kCentred, 3>(lo), codes_fp16<kCentred, 2>(hi), codes_fp16<kCentred, 3>(hi)};
+            float mn0 = Kv4Type<T>::hi(e0[g]), mn1 = Kv4Type<T>::hi(e1[g]);
+            if (kCentred) {
+              mn0 = fmaf(8.f, sc0[g], mn0);
+              mn1 = fmaf(8.f, sc1[g], mn1);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint32_t b0 = transpose8x8(Pack2<__half>::pack(pd[nt][0] * sc0[g], pd[nt][1] * sc0[g]));
+              const uint32_t b1 = transpose8x8(Pack2<__half>::pack(pd[nt][2] * sc1[g], pd[nt][3] * sc1[g]));
+              corr[nt][g][0] = fmaf(s[j][nt][0], mn0, fmaf(s[j][nt][2], mn1, corr[nt][g][0]));
+              corr[nt][g][1] = fmaf(s[j][nt][1], mn0, fmaf(s[j][nt][3], mn1, corr[nt][g][1]));
+              mma16816<__half>(o[nt][g][0], a0, b0, b1);
+              mma16816<__half>(o[nt][g][1], a1, b0, b1);
+            }
+          }
         }
       }
-      consumers_sync();  // the next run writes the same buffers
-      left -= run;
-      at.next_unit(p);
+      __syncwarp();
+      if (side == 1 && lane == 0) mbar_arrive(&bar_empty[pair][slot]);
     }
+
+    // ---- the four warps' results of this run into one ----
+    float* join = reinterpret_cast<float*>(smem + Cfg::kOffJoin);
+    float* ml = reinterpret_cast<float*>(smem + Cfg::kOffMl);
+    const float v_up = 1.f / v_down * 1048576.f;  // 2^20 of the odd codes; the even ones carry 2^4 more
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], d);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) corr[nt][g][x] += __shfl_xor_sync(0xffffffffu, corr[nt][g][x], d);
+        }
+        if (r == 0) {
+          ml[(warp * kRows + nt * 8 + 2 * c + x) * 2] = m[nt][x];
+          ml[(warp * kRows + nt * 8 + 2 * c + x) * 2 + 1] = l[nt][x];
+        }
+      }
+    __syncthreads();
+    float top[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        top[nt][x] = kNoKey;
+        for (int w = 0; w < 4; ++w) top[nt][x] = max_nan(top[nt][x], ml[(w * kRows + nt * 8 + 2 * c + x) * 2]);
+      }
+    for (int w = 0; w < 2; ++w) {  // in a fixed order: the same sum every time
+      if (w == side) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float f = fast_exp2(m[nt][x] - top[nt][x]);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {  // channels 32 g + 4 r + (0..3)
+              float4* dst = reinterpret_cast<float4*>(join + (pair * kRows + nt * 8 + 2 * c + x) * D + g * kGroup + 4 * r);
+              const float4 old = w == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *dst;
+              *dst = make_float4(fmaf(fmaf(o[nt][g][0][x], 16.f * v_up, corr[nt][g][x]), f, old.x),
+                                 fmaf(fmaf(o[nt][g][0][x + 2], v_up, corr[nt][g][x]), f, old.y),
+                                 fmaf(fmaf(o[nt][g][1][x], 16.f * v_up, corr[nt][g][x]), f, old.z),
+                                 fmaf(fmaf(o[nt][g][1][x + 2], v_up, corr[nt][g][x]), f, old.w));
+            }
+          }
+      }
+      __syncthreads();
+    }
+    const bool whole = at.page == 0 && run == at.pages;
+    const int slot = 2 * blockIdx.x + (at.page > 0 ? 0 : 1);
+    if (threadIdx.x == 0) {
+      int2* by = p.shared_by + static_cast<size_t>(at.b) * p.units + at.u;
+      if (at.page == 0) by->x = blockIdx.x;
+      if (at.page + run == at.pages) by->y = blockIdx.x;
+    }
+    for (int i = threadIdx.x; i < kRows * D / 8; i += 128) {
+      const int row = i / (D / 8), ch = i % (D / 8) * 8, rg = row0 + row;
+      if (rg >= n_rows) continue;
+      float mm = kNoKey, ll = 0.f;
+      for (int w = 0; w < 4; ++w) mm = max_nan(mm, ml[(w * kRows + row) * 2]);
+      for (int w = 0; w < 4; ++w) ll += ml[(w * kRows + row) * 2 + 1] * fast_exp2(ml[(w * kRows + row) * 2] - mm);
+      const float* even = join + row * D + ch;
+      const float* odd = even + kRows * D;
+      const float4 x = add4(*reinterpret_cast<const float4*>(even), *reinterpret_cast<const float4*>(odd));
+      const float4 y = add4(*reinterpret_cast<const float4*>(even + 4), *reinterpret_cast<const float4*>(odd + 4));
+      if (whole) {
+        const int t = rg / G, h = head * G + rg % G;
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        T* dst = static_cast<T*>(p.out) + ((static_cast<size_t>(at.b) * p.T + t) * p.Hq + h) * D + ch;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(Pack2<T>::pack(x.x * inv, x.y * inv), Pack2<T>::pack(x.z * inv, x.w * inv),
+                                                    Pack2<T>::pack(y.x * inv, y.y * inv), Pack2<T>::pack(y.z * inv, y.w * inv));
+        if (p.lse && ch == 0)
+          p.lse[(static_cast<size_t>(at.b) * p.Hq + h) * p.T + t] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) / kLog2e;
+      } else {
+        float* dst = p.part_o + (static_cast<size_t>(slot) * kRows + row) * D + ch;
+        *reinterpret_cast<float4*>(dst) = x;
+        *reinterpret_cast<float4*>(dst + 4) = y;
+        if (ch == 0) *reinterpret_cast<float2*>(p.part_ml + (static_cast<size_t>(slot) * kRows + row) * 2) = make_float2(mm, ll);
+      }
+    }
+    __syncthreads();  // the next run writes the same buffers
+    at.next_unit(p);
   }
-  __syncthreads();
   if (threadIdx.x == 0 && abort_flag) {
     // Give copies that are still in flight time to land before the block's shared memory is released.
     const unsigned long long t0 = global_timer_ns();
@@ -716,8 +876,7 @@ __global__ void __launch_bounds__(160, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
 // without keys.
 template <typename T>
 __global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttnParams p, int tile_rows) {
-  __shared__ long long red[2 * 4];
-  pdl_wait();
+  // what does not depend on the other kernel comes before the wait for it (it has waited for the lengths itself)
   const int n_row_tiles = p.units / p.Hkv, G = p.Hq / p.Hkv;
   const int row = blockIdx.x % tile_rows;
   const int u = blockIdx.x / tile_rows % p.units, b = blockIdx.x / tile_rows / p.units;
@@ -727,42 +886,67 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttnParams p, in
   T* dst = static_cast<T*>(p.out) + ((static_cast<size_t>(b) * p.T + t) * p.Hq + h) * p.D;
   float* lse = p.lse ? p.lse + (static_cast<size_t>(b) * p.Hq + h) * p.T + t : nullptr;
   const int pages = pages_of(kv4_len(p, b));
-  const int d = threadIdx.x * 2;
+  pdl_wait();
   if (pages == 0) {
-    if (d < p.D) *reinterpret_cast<uint32_t*>(dst + d) = 0;
-    if (lse && d == 0) *lse = -INFINITY;
+    if (threadIdx.x < p.D / 2) reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = 0;
+    if (lse && threadIdx.x == 0) *lse = -INFINITY;
     return;
   }
-  long long first;
-  const long long total = kv4_total(p, b, red, &first);
-  const long long quota = (total + p.blocks - 1) / p.blocks;
-  first += static_cast<long long>(u) * pages;
-  const int c0 = static_cast<int>(first / quota), c1 = static_cast<int>((first + pages - 1) / quota);
-  if (c0 == c1) return;  // written by that block
-  auto slot = [&](int c) { return static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * tile_rows + row; };
+  const int2 by = p.shared_by[static_cast<size_t>(b) * p.units + u];
+  const int c0 = by.x, c1 = by.y;
+  if (c0 >= c1 || c0 < 0 || c1 >= p.blocks) return;  // written by the block itself (or the other kernel gave up)
+  // Maximum and weights of the parts first, by all threads; then each warp sums every fourth part, loads of
+  // several parts in flight (one thread per channel pair walking all parts took 29 us for 37 of them).
+  __shared__ float weight[kMaxParts];
+  __shared__ float4 sums[128];
+  __shared__ float stat[2 * 4];
+  const int parts = c1 - c0 + 1;
+  auto slot = [&](int i) { return static_cast<size_t>(2 * (c0 + i) + (i == 0 ? 1 : 0)) * tile_rows + row; };
   float top = kNoKey;
-  for (int c = c0; c <= c1; ++c) top = max_nan(top, p.part_ml[slot(c) * 2]);
-  float sum = 0.f, x = 0.f, y = 0.f;
-#pragma unroll 4
-  for (int c = c0; c <= c1; ++c) {
-    const size_t s = slot(c);
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + s * 2);
-    const float f = fast_exp2(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
-    if (d < p.D) {
-      const float2 v = *reinterpret_cast<const float2*>(p.part_o + s * p.D + d);
-      x = fmaf(v.x, f, x);
-      y = fmaf(v.y, f, y);
-    }
+  for (int i = threadIdx.x; i < parts; i += 128) top = max_nan(top, p.part_ml[slot(i) * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((threadIdx.x & 31) == 0) stat[threadIdx.x >> 5] = top;
+  __syncthreads();
+  top = max_nan(max_nan(stat[0], stat[1]), max_nan(stat[2], stat[3]));
+  float sum = 0.f;
+  for (int i = threadIdx.x; i < parts; i += 128) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2);
+    weight[i] = fast_exp2(ml.x - top);
+    sum = fmaf(ml.y, weight[i], sum);
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) stat[4 + (threadIdx.x >> 5)] = sum;
+  __syncthreads();
+  sum = (stat[4] + stat[5]) + (stat[6] + stat[7]);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if (d < p.D) *reinterpret_cast<uint32_t*>(dst + d) = Pack2<T>::pack(x * inv, y * inv);
-  if (lse && d == 0) *lse = sum == 0.f ? -INFINITY : (top + log2f(sum)) / kLog2e;
+  if (lse && threadIdx.x == 0) *lse = sum == 0.f ? -INFINITY : (top + log2f(sum)) / kLog2e;
+  // a warp for every fourth part, lanes of 4 channels (two rounds for head dims above 128)
+  for (int d0 = 0; d0 < p.D; d0 += 128) {
+    const int d = d0 + (threadIdx.x & 31) * 4;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (d < p.D) {
+#pragma unroll 4
+      for (int i = threadIdx.x >> 5; i < parts; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p.part_o + slot(i) * p.D + d);
+        const float w = weight[i];
+        x = make_float4(fmaf(v.x, w, x.x), fmaf(v.y, w, x.y), fmaf(v.z, w, x.z), fmaf(v.w, w, x.w));
+      }
+    }
+    sums[threadIdx.x] = x;
+    __syncthreads();
+    if (threadIdx.x < 32 && d < p.D) {
+      x = add4(add4(sums[threadIdx.x], sums[threadIdx.x + 32]), add4(sums[threadIdx.x + 64], sums[threadIdx.x + 96]));
+      *reinterpret_cast<uint2*>(dst + d) = make_uint2(Pack2<T>::pack(x.x * inv, x.y * inv), Pack2<T>::pack(x.z * inv, x.w * inv));
+    }
+    __syncthreads();
+  }
 }
 
 // Column tiles of 8 query rows: two where there are more rows than one holds and registers for both.
 static int kv4_tiles(int T, int G, int D) { return T * G > 8 && D <= 128 ? 2 : 1; }
-static int kv4_blocks(int D, int nt) { return kSmCount * (D / kGroup * nt <= 4 ? 3 : 2); }
+static int kv4_blocks(int D, int nt) { return kSmCount * (D / kGroup * nt <= 4 ? 4 : D / kGroup * nt <= 6 ? 3 : 2); }
 static bool kv4_dim(int D) { return D == 64 || D == 96 || D == 128 || D == 192 || D == 256; }
 
 template <typename T, int NG, int NT>
@@ -779,7 +963,7 @@ static int launch_kv4_attn(const Kv4AttnParams& p, cudaStream_t s) {
     }
     attr_done[dev] = true;
   }
-  const int rc = launch_chained(kern, static_cast<unsigned>(p.blocks), 160, Cfg::kSmemBytes, s, p);
+  const int rc = launch_chained(kern, static_cast<unsigned>(p.blocks), 128, Cfg::kSmemBytes, s, p);
   if (rc != RFA_OK) return rc;
   return launch_chained(kv4_join_kernel<T>, static_cast<unsigned>(p.B) * p.units * Cfg::kRows, 128, 0, s, p,
                         static_cast<int>(Cfg::kRows));
@@ -860,11 +1044,12 @@ extern "C" int rfa_kv4_gather(void* k, void* v, const void* codes, const void* m
   return launch_chained(kv4_gather_kernel<__half>, grid, 256, 0, s, static_cast<__half*>(k), static_cast<__half*>(v), p, lanes);
 }
 
-extern "C" size_t rfa_kv4_scratch_elems(int T, int Hq, int Hkv, int D) {
+extern "C" size_t rfa_kv4_scratch_elems(int B, int T, int Hq, int Hkv, int D) {
   using namespace rfa;
-  if (T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || !kv4_dim(D)) return 0;
+  if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || !kv4_dim(D)) return 0;
   const int nt = kv4_tiles(T, Hq / Hkv, D);
-  return static_cast<size_t>(2) * kv4_blocks(D, nt) * 8 * nt * (D + 2);
+  const size_t units = (static_cast<size_t>(T) * (Hq / Hkv) + 8 * nt - 1) / (8 * nt) * Hkv;
+  return static_cast<size_t>(2) * kv4_blocks(D, nt) * 8 * nt * (D + 2) + 2 * units * B;
 }
 
 extern "C" int rfa_kv4_attn(const void* q, const long long* q_strides, const void* codes, const void* meta, int n_pages,
@@ -907,12 +1092,13 @@ extern "C" int rfa_kv4_attn(const void* q, const long long* q_strides, const voi
   p.n_pages = n_pages;
   p.max_pages = max_pages;
   p.units = static_cast<int>(units);
-  // no more blocks than pages there can be; a block's share must fit an int
+  // no more blocks than pages there can be; all of the work is counted in an int
   const long long most = static_cast<long long>(max_pages) * units * B;
+  if ((static_cast<long long>(max_pages) + kUnitCost) * units * B > INT_MAX) return RFA_ERR_TOO_LARGE;
   p.blocks = static_cast<int>(most < kv4_blocks(D, nt) ? most : kv4_blocks(D, nt));
-  if (most / p.blocks >= INT_MAX) return RFA_ERR_TOO_LARGE;
   p.part_o = scratch;
   p.part_ml = scratch + static_cast<size_t>(2) * p.blocks * rows * D;
+  p.shared_by = reinterpret_cast<int2*>(p.part_ml + static_cast<size_t>(2) * p.blocks * rows * 2);
   p.scale_log2 = softmax_scale * kLog2e;
   p.cap_log2 = softcap * kLog2e;
   p.cap_in = softcap > 0.f ? 2.f * softmax_scale * kLog2e / softcap : 0.f;

@@ -177,7 +177,7 @@ def _attn(q, cache, block_table, lens, softmax_scale, softcap, alibi_slopes, wan
     out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
     lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if want_lse else None
     # scratch per call: calls on several streams, or in several captured graphs, do not meet in it
-    scratch = torch.empty(_native.kv4_scratch_elems(T, Hq, cache.n_kv_heads, D), dtype=torch.float32, device=q.device)
+    scratch = torch.empty(_native.kv4_scratch_elems(B, T, Hq, cache.n_kv_heads, D), dtype=torch.float32, device=q.device)
     _native.kv4_attn(_rows(q.detach()), cache.codes, cache.meta, table, lens, out, lse, scratch, scale, softcap, slopes,
                      ws.status)
     workspace.publish_status(ws, "kv4_attn")

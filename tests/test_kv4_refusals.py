@@ -88,5 +88,8 @@ def test_abi_refuses_bad_arguments():
         256, st, 256, 256, 4, 256, 2, 256, 256, None, scratch, 1, T, Hq, 2, D, 0, scale, cap, None, 0, 256, None)
     assert att(Hq=3) == -1 and att(scale=0.0) == -1 and att(cap=-1.0) == -1 and att(scratch=None) == -1 and att(D=48) == -2
     assert att(T=1 << 30) == -5
-    assert lib.rfa_kv4_scratch_elems(1, 4, 3, 64) == 0 and lib.rfa_kv4_scratch_elems(1, 4, 2, 80) == 0
-    assert lib.rfa_kv4_scratch_elems(1, 4, 2, 128) >= 2 * 148 * 8 * 130
+    assert lib.rfa_kv4_scratch_elems(1, 1, 4, 3, 64) == 0 and lib.rfa_kv4_scratch_elems(1, 1, 4, 2, 80) == 0
+    assert lib.rfa_kv4_scratch_elems(0, 1, 4, 2, 64) == 0
+    # two parts of 8 rows per block at least, and two numbers per unit
+    assert lib.rfa_kv4_scratch_elems(5, 1, 4, 2, 128) - lib.rfa_kv4_scratch_elems(4, 1, 4, 2, 128) == 2 * 2
+    assert lib.rfa_kv4_scratch_elems(1, 1, 4, 2, 128) >= 2 * 148 * 8 * 130
