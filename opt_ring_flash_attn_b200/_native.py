@@ -10,8 +10,9 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from pathlib import Path
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -266,9 +267,9 @@ def scored_fwd_hop(q, k, v, acc, m, l, out, lse, args: ScoreArgs, first: bool, l
     """:func:`fwd_hop` with modified scores (``rfa_scored_fwd_hop``)."""
     B, S, Hq, D = q.shape
     with _on_device(q):
-        rc = load().rfa_scored_fwd_hop(_ptr(q), _ptr(k), _ptr(v), _ptr(acc), _ptr(m), _ptr(l), _ptr(out), _ptr(lse),
-                                       B, S, Hq, k.shape[2], D, DTYPE_CODES[q.dtype], ctypes.byref(args), int(first),
-                                       int(last), _ptr(status), _stream(stream, q))
+        rc = load().rfa_scored_fwd_hop(q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(acc), _ptr(m), _ptr(l), out.data_ptr(),
+                                       lse.data_ptr(), B, S, Hq, k.shape[2], D, DTYPE_CODES[q.dtype], ctypes.byref(args),
+                                       int(first), int(last), status.data_ptr(), _stream(stream, q))
     _check(rc, "rfa_scored_fwd_hop")
 
 
@@ -284,40 +285,63 @@ def scored_bwd_hop(q, k, v, dout, lse2, delta, dq_acc, dkdv_out, args: ScoreArgs
     _check(rc, "rfa_scored_bwd_hop")
 
 
-def scored_bwd_local(q, k, v, out, dout, lse, delta, lse2, dq_acc, dkdv, dq, dk, dv, args: ScoreArgs, status, stream=None,
-                     dq_order: Optional[torch.Tensor] = None) -> None:
-    """:func:`bwd_local` with modified scores (``rfa_scored_bwd_local``)."""
+def _aligned4(n: int) -> int:
+    return (n + 3) // 4 * 4
+
+
+@functools.lru_cache(maxsize=256)
+def scored_bwd_scratch(B: int, S: int, Hq: int, Hkv: int, D: int, deterministic: bool) -> Tuple[int, ...]:
+    """Float offsets of delta, lse2, dq_acc, dkdv and the ordering counters inside one buffer, and its size."""
+    rows = B * Hq * padded_seq(S)  # a multiple of 128
+    at = [0, rows, 2 * rows]
+    at.append(at[-1] + dq_acc_elems(B, S, Hq, D))
+    at.append(at[-1] + _aligned4(2 * B * S * Hkv * D))
+    at.append(at[-1] + (_aligned4(dq_order_elems(B, S, Hq, D)) if deterministic else 0))
+    return tuple(at)
+
+
+def scored_bwd_local(q, k, v, out, dout, lse, scratch, offsets, dq, dk, dv, args: ScoreArgs, status, stream=None,
+                     deterministic: bool = False) -> None:
+    """:func:`bwd_local` with modified scores (``rfa_scored_bwd_local``); ``scratch`` is one fp32 buffer with the parts at
+    ``offsets`` (:func:`scored_bwd_scratch`)."""
     B, S, Hq, D = q.shape
-    assert dq_order is None or (dq_order.dtype == torch.int32 and dq_order.numel() >= dq_order_elems(B, S, Hq, D))
+    base = scratch.data_ptr()
+    delta, lse2, dq_acc, dkdv, order = [base + 4 * o for o in offsets[:5]]
     with _on_device(q):
         rc = load().rfa_scored_bwd_local(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(dout), _ptr(lse), _ptr(delta), _ptr(lse2), _ptr(dq_acc), _ptr(dkdv),
-            _ptr(dq), _ptr(dk), _ptr(dv), B, S, Hq, k.shape[2], D, DTYPE_CODES[q.dtype], ctypes.byref(args),
-            _ptr(dq_order), _ptr(status), _stream(stream, q))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), delta, lse2, dq_acc,
+            dkdv, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, S, Hq, k.shape[2], D, DTYPE_CODES[q.dtype],
+            ctypes.byref(args), order if deterministic else None, status.data_ptr(), _stream(stream, q))
     _check(rc, "rfa_scored_bwd_local", kernels=3)
 
 
+_Strides = ctypes.c_longlong * 3
+
+
 def _strides(t: torch.Tensor):
-    return (ctypes.c_longlong * 3)(*t.stride()[:3])
+    st = t.stride()
+    return _Strides(st[0], st[1], st[2])
 
 
 def kv4_append(k, v, codes, meta, table, positions, counts, stream=None) -> None:
     B, T, Hkv, D = k.shape
     with _on_device(k):
-        rc = load().rfa_kv4_append(_ptr(k), _ptr(v), _strides(k), _strides(v), _ptr(codes), _ptr(meta), codes.shape[0],
-                                   _ptr(table), table.shape[1], _ptr(positions), _ptr(counts), B, T, Hkv, D,
-                                   DTYPE_CODES[meta.dtype], _stream(stream, k))
+        rc = load().rfa_kv4_append(k.data_ptr(), v.data_ptr(), _strides(k), _strides(v), codes.data_ptr(), meta.data_ptr(),
+                                   codes.shape[0], table.data_ptr(), table.shape[1], positions.data_ptr(), _ptr(counts), B, T,
+                                   Hkv, D, DTYPE_CODES[meta.dtype], _stream(stream, k))
     _check(rc, "rfa_kv4_append")
 
 
 def kv4_gather(k, v, codes, meta, table, positions, counts, stream=None) -> None:
     B, T, Hkv, D = k.shape
     with _on_device(k):
-        rc = load().rfa_kv4_gather(_ptr(k), _ptr(v), _ptr(codes), _ptr(meta), codes.shape[0], _ptr(table), table.shape[1],
-                                   _ptr(positions), _ptr(counts), B, T, Hkv, D, DTYPE_CODES[meta.dtype], _stream(stream, k))
+        rc = load().rfa_kv4_gather(k.data_ptr(), v.data_ptr(), codes.data_ptr(), meta.data_ptr(), codes.shape[0],
+                                   table.data_ptr(), table.shape[1], positions.data_ptr(), _ptr(counts), B, T, Hkv, D,
+                                   DTYPE_CODES[meta.dtype], _stream(stream, k))
     _check(rc, "rfa_kv4_gather")
 
 
+@functools.lru_cache(maxsize=256)
 def kv4_scratch_elems(B: int, T: int, Hq: int, Hkv: int, D: int) -> int:
     n = load().rfa_kv4_scratch_elems(B, T, Hq, Hkv, D)
     if n == 0:
@@ -329,10 +353,11 @@ def kv4_attn(q, codes, meta, table, lens, out, lse, scratch, softmax_scale: floa
              stream=None) -> None:
     B, T, Hq, D = q.shape
     with _on_device(q):
-        rc = load().rfa_kv4_attn(_ptr(q), _strides(q), _ptr(codes), _ptr(meta), codes.shape[0], _ptr(table), table.shape[1],
-                                 _ptr(lens), _ptr(out), _ptr(lse), _ptr(scratch), B, T, Hq, codes.shape[1], D,
-                                 DTYPE_CODES[q.dtype], softmax_scale, softcap, _ptr(slopes),
-                                 int(slopes is not None and slopes.dim() == 2), _ptr(status), _stream(stream, q))
+        rc = load().rfa_kv4_attn(q.data_ptr(), _strides(q), codes.data_ptr(), meta.data_ptr(), codes.shape[0],
+                                 table.data_ptr(), table.shape[1], lens.data_ptr(), out.data_ptr(), _ptr(lse),
+                                 scratch.data_ptr(), B, T, Hq, codes.shape[1], D, DTYPE_CODES[q.dtype], softmax_scale,
+                                 softcap, _ptr(slopes), int(slopes is not None and slopes.dim() == 2), status.data_ptr(),
+                                 _stream(stream, q))
     _check(rc, "rfa_kv4_attn", kernels=2)
 
 

@@ -43,6 +43,8 @@ class KV4Cache:
         if meta.device != codes.device:
             raise ValueError(f"codes are on {codes.device}, meta on {meta.device}")
         self.codes, self.meta = codes, meta
+        self.n_pages, self.n_kv_heads, self.head_dim = n, H, 2 * half
+        self.dtype, self.device = meta.dtype, codes.device
 
     @classmethod
     def empty(cls, n_pages: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
@@ -53,42 +55,22 @@ class KV4Cache:
         return cls(torch.empty(n_pages, n_kv_heads, 2, PAGE, head_dim // 2, dtype=torch.uint8, device=device),
                    torch.empty(n_pages, n_kv_heads, 2, PAGE, head_dim // GROUP, 2, dtype=dtype, device=device))
 
-    @property
-    def n_pages(self) -> int:
-        return self.codes.shape[0]
 
-    @property
-    def n_kv_heads(self) -> int:
-        return self.codes.shape[1]
-
-    @property
-    def head_dim(self) -> int:
-        return 2 * self.codes.shape[4]
-
-    @property
-    def dtype(self) -> torch.dtype:
-        return self.meta.dtype
-
-    @property
-    def device(self) -> torch.device:
-        return self.codes.device
-
-
-def _check_ints(x: Optional[torch.Tensor], shape: Tuple, device: torch.device, what: str) -> Optional[torch.Tensor]:
+def _check_ints(x: Optional[torch.Tensor], B: int, device: torch.device, what: str, dims: int = 1) -> Optional[torch.Tensor]:
     if x is None:
         return None
-    if x.dtype != torch.int32 or x.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, x.shape)):
-        want = ", ".join("n" if n is None else str(n) for n in shape)
-        raise ValueError(f"{what} must be int32 [{want}], got {x.dtype} {tuple(x.shape)}")
+    if x.dtype != torch.int32 or x.dim() != dims or x.shape[0] != B:
+        raise ValueError(f"{what} must be int32 [{B}{', n' if dims == 2 else ''}], got {x.dtype} {tuple(x.shape)}")
     if x.device != device:
         raise ValueError(f"{what} is on {x.device}, the cache on {device}")
-    return x.contiguous()
+    return x if x.is_contiguous() else x.contiguous()
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """The tensor itself where the kernels can read it as it lies (whole rows of channels on 16-byte boundaries, any strides
     of the other dimensions), else a copy."""
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:3]):
+    st = t.stride()
+    if st[3] == 1 and (st[0] | st[1] | st[2]) % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
@@ -126,13 +108,13 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, block_table: t
     if k.shape != v.shape:
         raise ValueError(f"k and v shapes differ: {tuple(k.shape)} vs {tuple(v.shape)}")
     B = k.shape[0]
-    table = _check_ints(block_table, (B, None), cache.device, "block_table")
-    positions = _check_ints(positions, (B,), cache.device, "positions")
-    counts = _check_ints(counts, (B,), cache.device, "counts")
+    table = _check_ints(block_table, B, cache.device, "block_table", 2)
+    positions = _check_ints(positions, B, cache.device, "positions")
+    counts = _check_ints(counts, B, cache.device, "counts")
     _check_cuda(cache)
     if k.numel() == 0 or table.shape[1] == 0:
         return
-    _native.kv4_append(_rows(k.detach()), _rows(v.detach()), cache.codes, cache.meta, table, positions, counts)
+    _native.kv4_append(_rows(k), _rows(v), cache.codes, cache.meta, table, positions, counts)
 
 
 def kv4_gather(cache: KV4Cache, block_table: torch.Tensor, positions: torch.Tensor, T: int,
@@ -142,9 +124,9 @@ def kv4_gather(cache: KV4Cache, block_table: torch.Tensor, positions: torch.Tens
     if T < 0:
         raise ValueError(f"T must not be negative, got {T}")
     B = block_table.shape[0]
-    table = _check_ints(block_table, (B, None), cache.device, "block_table")
-    positions = _check_ints(positions, (B,), cache.device, "positions")
-    counts = _check_ints(counts, (B,), cache.device, "counts")
+    table = _check_ints(block_table, B, cache.device, "block_table", 2)
+    positions = _check_ints(positions, B, cache.device, "positions")
+    counts = _check_ints(counts, B, cache.device, "counts")
     _check_cuda(cache)
     shape = (B, T, cache.n_kv_heads, cache.head_dim)
     if B == 0 or T == 0 or table.shape[1] == 0:
@@ -159,8 +141,8 @@ def _attn(q, cache, block_table, lens, softmax_scale, softcap, alibi_slopes, wan
     B, T, Hq, D = q.shape
     if Hq == 0 or Hq % cache.n_kv_heads != 0:
         raise ValueError(f"H_q must be a multiple of the cache's {cache.n_kv_heads} heads, got {Hq}")
-    table = _check_ints(block_table, (B, None), cache.device, "block_table")
-    lens = _check_ints(lens, (B,), cache.device, "lens")
+    table = _check_ints(block_table, B, cache.device, "block_table", 2)
+    lens = _check_ints(lens, B, cache.device, "lens")
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not (scale > 0) or math.isinf(scale):
         raise ValueError("softmax_scale must be positive and finite")
@@ -178,7 +160,7 @@ def _attn(q, cache, block_table, lens, softmax_scale, softcap, alibi_slopes, wan
     lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if want_lse else None
     # scratch per call: calls on several streams, or in several captured graphs, do not meet in it
     scratch = torch.empty(_native.kv4_scratch_elems(B, T, Hq, cache.n_kv_heads, D), dtype=torch.float32, device=q.device)
-    _native.kv4_attn(_rows(q.detach()), cache.codes, cache.meta, table, lens, out, lse, scratch, scale, softcap, slopes,
+    _native.kv4_attn(_rows(q), cache.codes, cache.meta, table, lens, out, lse, scratch, scale, softcap, slopes,
                      ws.status)
     workspace.publish_status(ws, "kv4_attn")
     return out, lse

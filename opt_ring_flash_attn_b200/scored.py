@@ -124,8 +124,16 @@ class _Scores:
         self.sees_later = sees_later  # some key behind a query may be visible: no hop can be left out
         self.world, self.rank, self._step = world, rank, 0
 
+        self._args = _native.score_args(softmax_scale, softcap, slopes, causal, mask_buffer, world, rank, rank)
+
+    def again(self) -> "_Scores":
+        """For another pass: the backward may run on another thread, and more than once."""
+        return self if self.world == 1 else _Scores(self.scale, self.softcap, self.slopes, self.causal, self.mask,
+                                                    self.sees_later, self.world, self.rank)
+
     def args(self, k_shard: int) -> _native.ScoreArgs:
-        return _native.score_args(self.scale, self.softcap, self.slopes, self.causal, self.mask, self.world, self.rank, k_shard)
+        self._args.k_shard = k_shard
+        return self._args
 
     def _next(self) -> _native.ScoreArgs:
         shard = (self.rank - self._step) % self.world  # a schedule runs its hops in the order of the steps
@@ -170,40 +178,37 @@ def _backward(group, dout, q, k, v, out, lse, sc: _Scores, deterministic: bool):
     ws = workspace.status_workspace(q.device)
     workspace.raise_if_failed(ws, "scored_flash_attn backward")
     B, S, Hq, D = q.shape
-    f32 = dict(dtype=torch.float32, device=q.device)
-    delta, lse2 = torch.empty_like(lse), torch.empty_like(lse)
-    dq_acc = torch.empty(_native.dq_acc_elems(B, S, Hq, D), **f32)
-    dkdv = torch.empty((2, *k.shape), **f32)
-    order = torch.empty(_native.dq_order_elems(B, S, Hq, D), dtype=torch.int32, device=q.device) if deterministic else None
+    offsets = _native.scored_bwd_scratch(B, S, Hq, k.shape[2], D, deterministic)
+    scratch = torch.empty(offsets[5], dtype=torch.float32, device=q.device)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    _native.scored_bwd_local(q, k, v, out, dout, lse, delta, lse2, dq_acc, dkdv, dq, dk, dv, sc.args(0), ws.status,
-                             dq_order=order)
+    _native.scored_bwd_local(q, k, v, out, dout, lse, scratch, offsets, dq, dk, dv, sc.args(0), ws.status,
+                             deterministic=deterministic)
     workspace.publish_status(ws, "scored_flash_attn backward")
     return dq, dk, dv
 
 
 def _operand(t: torch.Tensor) -> torch.Tensor:
     """Contiguous, and on the 16-byte boundary that the copies of the kernels start on."""
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _call(q, k, v, sc: _Scores, group):
+    """The forward pass on operands as the kernels want them."""
+    if q.numel() == 0:
+        return torch.empty_like(q), q.new_empty((q.shape[0], q.shape[2], 0), dtype=torch.float32)
+    return _forward(group, q, k, v, sc)
 
 
 class _ScoredFlashAttnFunc(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, softmax_scale, softcap, slopes, causal, mask, group):
-        world, rank = schedule._world(group)
-        sees_later = not causal or (mask is not None and mask.has_prefix)
-        buffer = None if mask is None else mask.buffer
+    def forward(ctx, q, k, v, sc, group):
         q, k, v = _operand(q), _operand(k), _operand(v)
-        ctx.args = (softmax_scale, softcap, causal, sees_later, world, rank)
-        ctx.group = group
+        out, lse = _call(q, k, v, sc, group)
+        ctx.sc, ctx.group = sc, group
         ctx.deterministic = _deterministic_now()
-        if q.numel() == 0:
-            out, lse = torch.empty_like(q), q.new_empty((q.shape[0], q.shape[2], 0), dtype=torch.float32)
-        else:
-            sc = _Scores(softmax_scale, softcap, slopes, causal, buffer, sees_later, world, rank)
-            out, lse = _forward(group, q, k, v, sc)
-        ctx.save_for_backward(q, k, v, out, lse, slopes, buffer)
+        ctx.save_for_backward(q, k, v, out, lse)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return out, lse
@@ -211,13 +216,11 @@ class _ScoredFlashAttnFunc(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, _dlse=None):
-        q, k, v, out, lse, slopes, buffer = ctx.saved_tensors
+        q, k, v, out, lse = ctx.saved_tensors
         if dout is None or q.numel() == 0:
-            return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), *[None] * 6)
-        scale, softcap, causal, sees_later, world, rank = ctx.args
-        sc = _Scores(scale, softcap, slopes, causal, buffer, sees_later, world, rank)
-        dq, dk, dv = _backward(ctx.group, _operand(dout), q, k, v, out, lse, sc, ctx.deterministic)
-        return (dq, dk, dv, *[None] * 6)
+            return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), None, None
+        dq, dk, dv = _backward(ctx.group, _operand(dout), q, k, v, out, lse, ctx.sc.again(), ctx.deterministic)
+        return dq, dk, dv, None, None
 
 
 def _check_slopes(slopes: Optional[torch.Tensor], B: int, Hq: int, device: torch.device) -> Optional[torch.Tensor]:
@@ -255,8 +258,8 @@ def _apply(q, k, v, softmax_scale, causal, softcap, alibi_slopes, mask, group) -
     softcap = _check_softcap(softcap)
     slopes = _check_slopes(alibi_slopes, B, Hq, q.device)
     causal = bool(causal)
+    world, rank = schedule._world(group)
     if mask is not None:
-        world, _ = schedule._world(group)
         if not isinstance(mask, DocumentMask):
             raise ValueError("mask must come from document_mask")
         if mask.causal != causal:
@@ -266,7 +269,11 @@ def _apply(q, k, v, softmax_scale, causal, softcap, alibi_slopes, mask, group) -
         if (mask.batch, mask.seq_len, mask.shards) != (B, S * world, world):
             raise ValueError(f"the mask is for a batch of {mask.batch} and {mask.seq_len} tokens on {mask.shards} ranks, "
                              f"the call has {B}, {S * world} and {world}")
-    return _ScoredFlashAttnFunc.apply(q, k, v, float(softmax_scale), softcap, slopes, causal, mask, group)
+    sees_later = not causal or (mask is not None and mask.has_prefix)
+    sc = _Scores(float(softmax_scale), softcap, slopes, causal, None if mask is None else mask.buffer, sees_later, world, rank)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _ScoredFlashAttnFunc.apply(q, k, v, sc, group)
+    return _call(_operand(q), _operand(k), _operand(v), sc, group)
 
 
 def scored_flash_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: Optional[float] = None,

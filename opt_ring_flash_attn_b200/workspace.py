@@ -154,13 +154,13 @@ _STATUS_CHECK = os.environ.get("RFA_B200_STATUS_CHECK", "1") != "0"
 
 def publish_status(ws, what: str) -> None:
     """End of a pass: enqueue the 4-byte copy of the status word to pinned host memory (``rfa_status_publish``)."""
-    if ws.status_host is None or not _STATUS_CHECK or _capturing(ws):
+    if ws.status_host is None or not _STATUS_CHECK:
         return
     sync = os.environ.get("RFA_B200_SYNC_STATUS", "0") == "1"
     # The copy costs the host some 15 microseconds, which is a tenth of a short-shard step: passes that follow each
     # other within a millisecond share one copy (a failure then surfaces a few passes later instead of one).
     now = time.perf_counter()
-    if not sync and now - ws.last_publish < 1e-3:
+    if (not sync and now - ws.last_publish < 1e-3) or _capturing(ws):
         return
     ws.last_publish = now
     if ws.status_event is None:
