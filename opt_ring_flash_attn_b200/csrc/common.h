@@ -69,13 +69,13 @@ inline int cuda_status(cudaError_t e) {
 // pdl_wait() before it touches global memory, so that what it reads is complete and what it overwrites is no longer
 // read; what comes before (barriers, tensor memory, descriptors) overlaps the predecessor's tail.
 template <typename... P, typename... A>
-inline int launch_chained(void (*kern)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream,
+inline int launch_chained(void (*kern)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
                           const A&... args) {
   cudaLaunchAttribute attr[1] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;

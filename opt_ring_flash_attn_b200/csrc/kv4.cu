@@ -8,6 +8,8 @@
 // channels, channels [32 g + 8 c, + 8) at word c * NG + g; V as half words of 4, [32 g + 4 c, + 4) at c * NG + g.
 #include <limits.h>
 
+#include <type_traits>
+
 #include "scored.cuh"
 
 namespace rfa {
@@ -37,6 +39,15 @@ struct Kv4Type<__half> {
   static __device__ __forceinline__ float hi(uint32_t w) { return value(static_cast<uint16_t>(w >> 16)); }
 };
 
+// Larger ones of two pairs; NaN where either is.
+template <typename T>
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (Pack2<T>::kIsBf16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 struct Kv4Pages {
   uint8_t* codes;
   void* meta;
@@ -57,78 +68,111 @@ __device__ __forceinline__ long long kv4_row(const Kv4Pages& p, int b, int t, in
   return ((static_cast<long long>(page) * p.Hkv + h) * 2) * kPage + pos % kPage;
 }
 
+// The code of an x that lies next to a border between two (16-bit inputs hit borders exactly, about one in a thousand): the
+// sign of x - lo - border * sc decides.  The product is exact (5 bits times 11), its difference from x - lo is (they are nearly
+// equal), and what rounding x - lo left over is known.  A call, because unrolled into its caller it outgrows the instruction
+// cache.
+__device__ __noinline__ float border_code(float x, float lo, float sc, float t) {
+  const float d = x - lo;
+  const float below = floorf(t), border = below + 0.5f;
+  const float part_x = d + lo, part_lo = d - part_x;  // d = x - lo + what the two parts lack
+  const float left = (x - part_x) + (-lo - part_lo);
+  const float side = fmaf(-border, sc, d) + left;
+  const bool up = side > 0.f || (side == 0.f && (static_cast<int>(below) & 1));
+  return fminf(up ? below + 1.f : below, 15.f);
+}
+
 // Codes of 8 channels (one lane), low bits first, and the group's (sc, min) in T's bits.
 template <typename T>
 __device__ __forceinline__ uint32_t quantize8(const uint4& raw, uint32_t& meta) {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = Kv4Type<T>::lo(w[i]);
-    x[2 * i + 1] = Kv4Type<T>::hi(w[i]);
-  }
-  // a NaN anywhere makes the group NaN, an infinity gives it an infinite scale: either way it does not read back as numbers
-  float hi = x[0], lo = -x[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    hi = max_nan(hi, x[i]);
-    lo = max_nan(lo, -x[i]);
-  }
-#pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    lo = max_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-  }
-  lo = -lo;
+  // Maximum and (negated) minimum as pairs of 16 bits.  A NaN anywhere makes the group NaN, an infinity gives it an infinite
+  // scale: either way it does not read back as numbers.
+  const uint32_t top2 = max2_nan<T>(max2_nan<T>(raw.x, raw.y), max2_nan<T>(raw.z, raw.w));
+  constexpr uint32_t sign = 0x80008000u;
+  const uint32_t low2 = max2_nan<T>(max2_nan<T>(raw.x ^ sign, raw.y ^ sign), max2_nan<T>(raw.z ^ sign, raw.w ^ sign));
+  uint32_t ends = max2_nan<T>(__byte_perm(top2, low2, 0x5410), __byte_perm(top2, low2, 0x7632));  // (max, -min)
+  ends = max2_nan<T>(ends, __shfl_xor_sync(0xffffffffu, ends, 1));
+  ends = max2_nan<T>(ends, __shfl_xor_sync(0xffffffffu, ends, 2));
+  const float hi = Kv4Type<T>::lo(ends);
+  float lo = -Kv4Type<T>::hi(ends);
   const uint16_t sb = Kv4Type<T>::bits((hi - lo) / 15.f);
-  const float sc = Kv4Type<T>::value(sb);
-  meta = static_cast<uint32_t>(sb) | (static_cast<uint32_t>(Kv4Type<T>::bits(lo)) << 16);
+  float sc = Kv4Type<T>::value(sb);
+  meta = static_cast<uint32_t>(sb) | ((ends ^ sign) & 0xffff0000u);
   if (!(sc > 0.f)) return 0;
+  float x[8] = {Kv4Type<T>::lo(raw.x), Kv4Type<T>::hi(raw.x), Kv4Type<T>::lo(raw.y), Kv4Type<T>::hi(raw.y),
+                Kv4Type<T>::lo(raw.z), Kv4Type<T>::hi(raw.z), Kv4Type<T>::lo(raw.w), Kv4Type<T>::hi(raw.w)};
+  if (sc < 1e-30f) {  // its reciprocal would leave fp32 (bf16 only): the same codes under a power of two
+    constexpr float up = 18446744073709551616.f;
+    sc *= up;
+    lo *= up;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= up;
+  }
+  // (x - lo) * (1 / sc) is off by less than 3e-6 in 15, so its nearest whole number is the code unless it lies within 1e-5
+  // of a border between two codes.
   const float inv = 1.f / sc;
-  uint32_t codes = 0;
+  constexpr float magic = 12582912.f;  // 1.5 * 2^23: adding it rounds to a whole number, ties to even
+  float u[8], away = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    // (x - lo) * (1 / sc) is off by less than 3e-6 in 15; where it lies within 1e-5 of a border between two codes the
-    // quotient itself decides, in 64 bits (16-bit inputs hit borders exactly, about one in a thousand)
-    float t = (x[i] - lo) * inv;
-    if (fabsf(fabsf(t - floorf(t)) - 0.5f) < 1e-5f) t = static_cast<float>(rint((static_cast<double>(x[i]) - lo) / sc));
-    const int u = __float2int_rn(fminf(fmaxf(t, 0.f), 15.f));
-    codes |= static_cast<uint32_t>(u) << (4 * i);
+    const float t = fminf((x[i] - lo) * inv, 15.f);
+    u[i] = (t + magic) - magic;
+    away = fmaxf(away, fabsf(t - u[i]));
   }
-  return codes;
+  if (away > 0.49999f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float t = fminf((x[i] - lo) * inv, 15.f);
+      if (fabsf(t - u[i]) > 0.49999f) u[i] = border_code(x[i], lo, sc, t);
+    }
+  }
+  // four codes each, as a number of 16 bits
+  const float p0 = fmaf(fmaf(fmaf(u[3], 16.f, u[2]), 16.f, u[1]), 16.f, u[0]);
+  const float p1 = fmaf(fmaf(fmaf(u[7], 16.f, u[6]), 16.f, u[5]), 16.f, u[4]);
+  return static_cast<uint32_t>(__float2int_rn(p0)) | (static_cast<uint32_t>(__float2int_rn(p1)) << 16);
 }
 
-template <typename T>
+// Lane i of sequence b: channels [32 g + 8 c, + 8) of head h of token t, in the order of memory.
+template <int NG>
+struct Kv4Lane {
+  int c, g, h, t;
+  __device__ __forceinline__ Kv4Lane(unsigned i, unsigned Hkv) {
+    c = i & 3;
+    const unsigned group = i >> 2, row = group / NG;
+    g = group % NG;
+    h = row % Hkv;
+    t = row / Hkv;
+  }
+};
+
+template <typename T, int NG>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k, const T* __restrict__ v, Kv4Pages p,
-                                                         longlong3 ks, longlong3 vs, long long lanes) {
+                                                         longlong3 ks, longlong3 vs, unsigned lanes) {
   pdl_wait();
-  const int NG = p.D / kGroup;
-  const long long id = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  pdl_trigger();  // what follows on the stream waits for the results itself
+  const unsigned id = blockIdx.x * 256u + threadIdx.x;
   const bool in = id < lanes;
-  const long long i = in ? id : 0;
-  const int c = static_cast<int>(i & 3);
-  const int g = static_cast<int>((i >> 2) % NG);
-  const long long row = (i >> 2) / NG;
-  const int h = static_cast<int>(row % p.Hkv);
-  const int t = static_cast<int>(row / p.Hkv % p.T);
-  const int b = static_cast<int>(row / p.Hkv / p.T);
+  const Kv4Lane<NG> at_lane(in ? id : 0, p.Hkv);
+  const int c = at_lane.c, g = at_lane.g;
   const int ch = g * kGroup + c * 8;
-  const uint4 kr = __ldg(reinterpret_cast<const uint4*>(k + b * ks.x + t * ks.y + h * ks.z + ch));
-  const uint4 vr = __ldg(reinterpret_cast<const uint4*>(v + b * vs.x + t * vs.y + h * vs.z + ch));
-  const long long at = kv4_row(p, b, t, h);
-  uint32_t km, vm;
-  const uint32_t kc = quantize8<T>(kr, km);
-  const uint32_t vc = quantize8<T>(vr, vm);
-  if (!in || at < 0) return;
-  const size_t half = p.D / 2;
-  uint8_t* kd = p.codes + at * half;
-  uint8_t* vd = kd + kPage * half;
-  *reinterpret_cast<uint32_t*>(kd + 4 * (c * NG + g)) = kc;
-  *reinterpret_cast<uint16_t*>(vd + 2 * (2 * c * NG + g)) = static_cast<uint16_t>(vc);
-  *reinterpret_cast<uint16_t*>(vd + 2 * ((2 * c + 1) * NG + g)) = static_cast<uint16_t>(vc >> 16);
-  uint32_t* md = static_cast<uint32_t*>(p.meta);
-  if (c == 0) md[at * NG + g] = km;
-  if (c == 1) md[(at + kPage) * NG + g] = vm;
+  constexpr size_t half = NG * kGroup / 2;
+  for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
+    const uint4 kr = __ldg(reinterpret_cast<const uint4*>(k + b * ks.x + at_lane.t * ks.y + at_lane.h * ks.z + ch));
+    const uint4 vr = __ldg(reinterpret_cast<const uint4*>(v + b * vs.x + at_lane.t * vs.y + at_lane.h * vs.z + ch));
+    const long long at = kv4_row(p, b, at_lane.t, at_lane.h);
+    uint32_t km, vm;
+    const uint32_t kc = quantize8<T>(kr, km);
+    const uint32_t vc = quantize8<T>(vr, vm);
+    if (!in || at < 0) continue;
+    uint8_t* kd = p.codes + at * half;
+    uint8_t* vd = kd + kPage * half;
+    *reinterpret_cast<uint32_t*>(kd + 4 * (c * NG + g)) = kc;
+    *reinterpret_cast<uint16_t*>(vd + 2 * (2 * c * NG + g)) = static_cast<uint16_t>(vc);
+    *reinterpret_cast<uint16_t*>(vd + 2 * ((2 * c + 1) * NG + g)) = static_cast<uint16_t>(vc >> 16);
+    uint32_t* md = static_cast<uint32_t*>(p.meta);
+    if (c == 0) md[at * NG + g] = km;
+    if (c == 1) md[(at + kPage) * NG + g] = vm;
+  }
 }
 
 template <typename T>
@@ -142,33 +186,31 @@ __device__ __forceinline__ uint4 dequantize8(uint32_t codes, uint32_t meta) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) kv4_gather_kernel(T* __restrict__ k, T* __restrict__ v, Kv4Pages p, long long lanes) {
+template <typename T, int NG>
+__global__ void __launch_bounds__(256) kv4_gather_kernel(T* __restrict__ k, T* __restrict__ v, Kv4Pages p, unsigned lanes) {
   pdl_wait();
-  const int NG = p.D / kGroup;
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const unsigned i = blockIdx.x * 256u + threadIdx.x;
   if (i >= lanes) return;
-  const int c = static_cast<int>(i & 3);
-  const int g = static_cast<int>((i >> 2) % NG);
-  const long long row = (i >> 2) / NG;
-  const int h = static_cast<int>(row % p.Hkv);
-  const int t = static_cast<int>(row / p.Hkv % p.T);
-  const int b = static_cast<int>(row / p.Hkv / p.T);
-  const long long at = kv4_row(p, b, t, h);
-  uint4 ko = make_uint4(0, 0, 0, 0), vo = ko;
-  if (at >= 0) {
-    const size_t half = p.D / 2;
-    const uint8_t* kd = p.codes + at * half;
-    const uint8_t* vd = kd + kPage * half;
-    const uint32_t* md = static_cast<const uint32_t*>(p.meta);
-    const uint32_t kc = *reinterpret_cast<const uint32_t*>(kd + 4 * (c * NG + g));
-    const uint32_t v0 = *reinterpret_cast<const uint16_t*>(vd + 2 * (2 * c * NG + g));
-    const uint32_t v1 = *reinterpret_cast<const uint16_t*>(vd + 2 * ((2 * c + 1) * NG + g));
-    ko = dequantize8<T>(kc, md[at * NG + g]);
-    vo = dequantize8<T>(v0 | (v1 << 16), md[(at + kPage) * NG + g]);
+  const Kv4Lane<NG> lane(i, p.Hkv);
+  const int c = lane.c, g = lane.g;
+  constexpr size_t half = NG * kGroup / 2;
+  for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
+    const long long at = kv4_row(p, b, lane.t, lane.h);
+    uint4 ko = make_uint4(0, 0, 0, 0), vo = ko;
+    if (at >= 0) {
+      const uint8_t* kd = p.codes + at * half;
+      const uint8_t* vd = kd + kPage * half;
+      const uint32_t* md = static_cast<const uint32_t*>(p.meta);
+      const uint32_t kc = *reinterpret_cast<const uint32_t*>(kd + 4 * (c * NG + g));
+      const uint32_t v0 = *reinterpret_cast<const uint16_t*>(vd + 2 * (2 * c * NG + g));
+      const uint32_t v1 = *reinterpret_cast<const uint16_t*>(vd + 2 * ((2 * c + 1) * NG + g));
+      ko = dequantize8<T>(kc, md[at * NG + g]);
+      vo = dequantize8<T>(v0 | (v1 << 16), md[(at + kPage) * NG + g]);
+    }
+    const size_t to = (static_cast<size_t>(b) * lanes + i) * 8;  // lanes run over [T][Hkv][D / 8]
+    *reinterpret_cast<uint4*>(k + to) = ko;
+    *reinterpret_cast<uint4*>(v + to) = vo;
   }
-  *reinterpret_cast<uint4*>(k + i * 8) = ko;  // lanes run over [B][T][Hkv][D / 8]
-  *reinterpret_cast<uint4*>(v + i * 8) = vo;
 }
 
 // ----------------------------------------------------------------------------
@@ -981,6 +1023,24 @@ static int dispatch_kv4_attn(const Kv4AttnParams& p, int nt, cudaStream_t s) {
   }
 }
 
+// f(a value of the 16-bit type, the number of channel groups)
+template <typename F>
+static int kv4_by_groups(int D, F&& f) {
+  switch (D / kGroup) {
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 3: return f(std::integral_constant<int, 3>{});
+    case 4: return f(std::integral_constant<int, 4>{});
+    case 6: return f(std::integral_constant<int, 6>{});
+    case 8: return f(std::integral_constant<int, 8>{});
+    default: return RFA_ERR_UNSUPPORTED;
+  }
+}
+template <typename F>
+static int kv4_by_type(int dtype, int D, F&& f) {
+  if (dtype == RFA_DTYPE_BF16) return kv4_by_groups(D, [&](auto groups) { return f(__nv_bfloat16{}, groups); });
+  return kv4_by_groups(D, [&](auto groups) { return f(__half{}, groups); });
+}
+
 static int kv4_check(const void* codes, const void* meta, int n_pages, const int* table, int max_pages, const int* rows, int B,
                      int T, int Hkv, int D, int dtype) {
   if (!codes || !meta || !table || !rows) return RFA_ERR_INVALID_ARG;
@@ -1008,18 +1068,18 @@ extern "C" int rfa_kv4_append(const void* k, const void* v, const long long* k_s
   if ((reinterpret_cast<uintptr_t>(k) & 15u) || (reinterpret_cast<uintptr_t>(v) & 15u) ||
       (reinterpret_cast<uintptr_t>(counts) & 3u))
     return RFA_ERR_INVALID_ARG;
-  const long long lanes = static_cast<long long>(B) * T * Hkv * (D / 8);
-  if (lanes > 256ll * INT_MAX) return RFA_ERR_TOO_LARGE;
+  if (static_cast<long long>(T) * Hkv * (D / 8) > INT_MAX - 256) return RFA_ERR_TOO_LARGE;
+  const unsigned lanes = static_cast<unsigned>(T) * Hkv * (D / 8);  // of a sequence
   const Kv4Pages p{static_cast<uint8_t*>(codes), meta, table, positions, counts, n_pages, max_pages, B, T, Hkv, D};
   const longlong3 ks = make_longlong3(k_strides[0], k_strides[1], k_strides[2]);
   const longlong3 vs = make_longlong3(v_strides[0], v_strides[1], v_strides[2]);
-  const unsigned grid = static_cast<unsigned>((lanes + 255) / 256);
+  const dim3 grid((lanes + 255) / 256, B < 65535 ? B : 65535);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == RFA_DTYPE_BF16)
-    return launch_chained(kv4_append_kernel<__nv_bfloat16>, grid, 256, 0, s, static_cast<const __nv_bfloat16*>(k),
-                          static_cast<const __nv_bfloat16*>(v), p, ks, vs, lanes);
-  return launch_chained(kv4_append_kernel<__half>, grid, 256, 0, s, static_cast<const __half*>(k),
-                        static_cast<const __half*>(v), p, ks, vs, lanes);
+  return kv4_by_type(dtype, D, [&](auto type, auto groups) {
+    using T16 = decltype(type);
+    return launch_chained(kv4_append_kernel<T16, decltype(groups)::value>, grid, 256, 0, s, static_cast<const T16*>(k),
+                          static_cast<const T16*>(v), p, ks, vs, lanes);
+  });
 }
 
 extern "C" int rfa_kv4_gather(void* k, void* v, const void* codes, const void* meta, int n_pages, const int* table,
@@ -1032,16 +1092,17 @@ extern "C" int rfa_kv4_gather(void* k, void* v, const void* codes, const void* m
   if ((reinterpret_cast<uintptr_t>(k) & 15u) || (reinterpret_cast<uintptr_t>(v) & 15u) ||
       (reinterpret_cast<uintptr_t>(counts) & 3u))
     return RFA_ERR_INVALID_ARG;
-  const long long lanes = static_cast<long long>(B) * T * Hkv * (D / 8);
-  if (lanes > 256ll * INT_MAX) return RFA_ERR_TOO_LARGE;
+  if (static_cast<long long>(T) * Hkv * (D / 8) > INT_MAX - 256) return RFA_ERR_TOO_LARGE;
+  const unsigned lanes = static_cast<unsigned>(T) * Hkv * (D / 8);  // of a sequence
   const Kv4Pages p{static_cast<uint8_t*>(const_cast<void*>(codes)), const_cast<void*>(meta), table, positions, counts,
                    n_pages, max_pages, B, T, Hkv, D};
-  const unsigned grid = static_cast<unsigned>((lanes + 255) / 256);
+  const dim3 grid((lanes + 255) / 256, B < 65535 ? B : 65535);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == RFA_DTYPE_BF16)
-    return launch_chained(kv4_gather_kernel<__nv_bfloat16>, grid, 256, 0, s, static_cast<__nv_bfloat16*>(k),
-                          static_cast<__nv_bfloat16*>(v), p, lanes);
-  return launch_chained(kv4_gather_kernel<__half>, grid, 256, 0, s, static_cast<__half*>(k), static_cast<__half*>(v), p, lanes);
+  return kv4_by_type(dtype, D, [&](auto type, auto groups) {
+    using T16 = decltype(type);
+    return launch_chained(kv4_gather_kernel<T16, decltype(groups)::value>, grid, 256, 0, s, static_cast<T16*>(k),
+                          static_cast<T16*>(v), p, lanes);
+  });
 }
 
 extern "C" size_t rfa_kv4_scratch_elems(int B, int T, int Hq, int Hkv, int D) {

@@ -113,6 +113,7 @@ def test_codes_and_values(D, dt):
     v[1, 2] *= 1e-6
     v[1, 3] *= 1e4
     v[2, 5] = v[2, 5].abs() * 1e-8
+    v[2, 6] *= 1e-38  # bf16: scales below the smallest normal number
     start = [130, 0, 60]
     before = cache.codes.clone(), cache.meta.clone()
     rfa.kv4_append(cache, k, v, table, _ints(start))
