@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(256) bwd_prepare_kernel(const T* __restrict__ 
     const int s = static_cast<int>(bs % Spad);
     const int b = static_cast<int>(bs / Spad);
     const size_t stat = (static_cast<size_t>(b) * Hq + h) * Spad + s;
-    const bool real = in_range && s < Sq;
+    // a row that saw no key (lse -inf: padding of a document mask, whose dout may be anything) has delta 0 and weights 0
+    const bool real = in_range && s < Sq && lse[stat] != -INFINITY;
     float acc = 0.f;
     if (real && gl < vec_per_row) {
       const size_t row_off = ((static_cast<size_t>(b) * Sq + s) * Hq + h) * D;

@@ -91,6 +91,86 @@ struct ScoredBwdCfg {
   static_assert(kSmemBytes <= 232448 - 1024, "shared memory over budget");
 };
 
+// What a CTA works on.  Worked out once and kept in shared memory: each role takes into registers what it needs.
+struct BwdPlan {
+  int kvt, hf, part, hkv, b;
+  int i_begin, n_i;          // query tiles that some key of the tile is seen by
+  int full_lo, full_hi;      // rows [full_lo, full_hi) of the query block see every key of the tile
+  int t0, t_total;           // this CTA's run of the G * n_i query tiles, head-major
+  int real_lo, real_hi;      // rows of the whole sequence that are no padding
+};
+// Query head and tile of step t of a run.
+struct BwdWalk {
+  int t0, n_i, i_begin, head0;
+  __device__ __forceinline__ BwdWalk(const BwdPlan& x, int G) : t0(x.t0), n_i(x.n_i), i_begin(x.i_begin), head0(x.hkv * G) {}
+  __device__ __forceinline__ int head(int t) const { return head0 + (t0 + t) / n_i; }
+  __device__ __forceinline__ int tile(int t) const { return i_begin + (t0 + t) % n_i; }
+};
+
+template <int DP, int DH, int BQ>
+__device__ __forceinline__ void make_plan(const ScoredBwdParams& prm, BwdPlan& plan) {
+  const BwdParams& p = prm.p;
+  const ScoreParams& sc = prm.sc;
+  constexpr int kHalves = DP / DH;
+  // Key tile first, so that the CTAs with the most visible queries start first (with a mask: in the order of its work list)
+  // and the tail of the grid evens out; blocks that every query sees go head group first, which keeps the dQ accumulator of
+  // the resident CTAs in L2.  The ordered mode needs key tiles in rising block order.
+  const bool worklist = sc.has_mask && p.dq_order == nullptr;
+  const int nkvt = (p.Skv + 127) / 128;
+  int kvt, hf, part, hkv, b;
+  {
+    int rem = static_cast<int>(blockIdx.x);
+    hf = rem % kHalves;
+    rem /= kHalves;
+    if (p.causal || sc.has_mask) {
+      part = rem % p.nsplit;  // CTAs that share a K/V tile are adjacent (the tile stays in L2)
+      rem /= p.nsplit;
+      hkv = rem % p.Hkv;
+      rem /= p.Hkv;
+      if (worklist) {
+        rem = __ldg(sc.mask.order_k + rem);
+        b = rem / nkvt;
+        kvt = rem % nkvt;
+      } else {
+        b = rem % p.B;
+        kvt = rem / p.B;
+      }
+    } else {
+      kvt = rem % nkvt;
+      rem /= nkvt;
+      part = rem % p.nsplit;
+      rem /= p.nsplit;
+      hkv = rem % p.Hkv;
+      b = rem / p.Hkv;
+    }
+  }
+  const int G = p.Hq / p.Hkv;
+  const int n0 = kvt * 128;
+  const int nQtiles = (p.Sq + BQ - 1) / BQ;
+  // Query rows of the block: [lo, hi) is the hull of what the keys of this tile are seen by, [full_lo, full_hi) what sees
+  // them all.  The ordered mode visits every tile of a masked block: its counters expect every key tile.
+  int i_begin, i_end, full_lo, full_hi;
+  {
+    const int4 hull = key_hull(sc, b, nkvt, kvt, p.Skv);
+    const int lo = max(hull.x - sc.q_pos, 0), hi = min(hull.w - sc.q_pos, p.Sq);
+    i_begin = lo / BQ;
+    i_end = lo < hi ? (hi + BQ - 1) / BQ : i_begin;
+    full_lo = max(hull.y, sc.q_pos) - sc.q_pos;
+    full_hi = hull.z - sc.q_pos;
+    if (sc.has_mask && !worklist) {
+      i_begin = 0;
+      i_end = nQtiles;
+    }
+  }
+  const int n_i = i_end - i_begin;
+  // The G * n_i query tiles of the K/V tile, head-major, are dealt out to nsplit CTAs in equal runs.
+  const int t0 = static_cast<int>(static_cast<long long>(G) * n_i * part / p.nsplit);
+  const int t_total = static_cast<int>(static_cast<long long>(G) * n_i * (part + 1) / p.nsplit) - t0;
+  const int real_lo = sc.has_mask ? __ldg(sc.mask.real + 2 * b) : 0;
+  const int real_hi = sc.has_mask ? __ldg(sc.mask.real + 2 * b + 1) : sc.len;
+  if ((threadIdx.x & 31) == 0) plan = BwdPlan{kvt, hf, part, hkv, b, i_begin, n_i, full_lo, full_hi, t0, t_total, real_lo, real_hi};
+}
+
 template <int DP, int DH, int BQ, int NSQ, int NSO, typename T, int kKind>
 __global__ void __launch_bounds__(640, 1)
     scored_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -108,6 +188,7 @@ __global__ void __launch_bounds__(640, 1)
   __shared__ uint64_t bar_q_full[NSQ], bar_q_empty[NSQ], bar_do_full[NSO], bar_do_empty[NSO];
   __shared__ uint64_t bar_s_full, bar_p_ready, bar_dp_full, bar_ds_ready, bar_dq_full, bar_dq_drained, bar_final;
   __shared__ uint32_t tmem_holder;
+  __shared__ BwdPlan plan;
   __shared__ int abort_flag, skip_flag;
 
   const int tid = threadIdx.x;
@@ -151,65 +232,7 @@ __global__ void __launch_bounds__(640, 1)
   }
   pdl_wait();  // nothing above touches global memory
 
-  // ---- tile coordinates ----
-  // Key tile first, so that the CTAs with the most visible queries start first (with a mask: in the order of its work list)
-  // and the tail of the grid evens out; blocks that every query sees go head group first, which keeps the dQ accumulator of
-  // the resident CTAs in L2.  The ordered mode needs key tiles in rising block order.
-  const bool worklist = sc.has_mask && p.dq_order == nullptr;
-  const int nkvt = (p.Skv + 127) / 128;
-  int kvt, hf, part, hkv, b;
-  {
-    int rem = static_cast<int>(blockIdx.x);
-    hf = rem % Cfg::kHalves;
-    rem /= Cfg::kHalves;
-    if (p.causal || sc.has_mask) {
-      part = rem % p.nsplit;  // CTAs that share a K/V tile are adjacent (the tile stays in L2)
-      rem /= p.nsplit;
-      hkv = rem % p.Hkv;
-      rem /= p.Hkv;
-      if (worklist) {
-        rem = __ldg(sc.mask.order_k + rem);
-        b = rem / nkvt;
-        kvt = rem % nkvt;
-      } else {
-        b = rem % p.B;
-        kvt = rem / p.B;
-      }
-    } else {
-      kvt = rem % nkvt;
-      rem /= nkvt;
-      part = rem % p.nsplit;
-      rem /= p.nsplit;
-      hkv = rem % p.Hkv;
-      b = rem / p.Hkv;
-    }
-  }
-  const int G = p.Hq / p.Hkv;
-  const int n0 = kvt * 128;
-  const int nQtiles = (p.Sq + BQ - 1) / BQ;
-  // Query rows of the block: [lo, hi) is the hull of what the keys of this tile are seen by, [full_lo, full_hi) what sees
-  // them all.  The ordered mode visits every tile of a masked block: its counters expect every key tile.
-  int i_begin, i_end, full_lo, full_hi;
-  {
-    const int4 hull = key_hull(sc, b, nkvt, kvt, p.Skv);
-    const int lo = max(hull.x - sc.q_pos, 0), hi = min(hull.w - sc.q_pos, p.Sq);
-    i_begin = lo / BQ;
-    i_end = lo < hi ? (hi + BQ - 1) / BQ : i_begin;
-    full_lo = max(hull.y, sc.q_pos) - sc.q_pos;
-    full_hi = hull.z - sc.q_pos;
-    if (sc.has_mask && !worklist) {
-      i_begin = 0;
-      i_end = nQtiles;
-    }
-  }
-  const int nI = i_end - i_begin;
-  // The G * nI query tiles of the K/V tile, head-major, are dealt out to nsplit CTAs in equal runs [t0, t0 + T_total).
-  const int t0 = static_cast<int>(static_cast<long long>(G) * nI * part / p.nsplit);
-  const int T_total = static_cast<int>(static_cast<long long>(G) * nI * (part + 1) / p.nsplit) - t0;
-  // rows of the whole sequence that are no padding
-  const int real_lo = sc.has_mask ? __ldg(sc.mask.real + 2 * b) : 0;
-  const int real_hi = sc.has_mask ? __ldg(sc.mask.real + 2 * b + 1) : sc.len;
-
+  if (warp == 0) make_plan<DP, DH, BQ>(prm, plan);
   if (tid == 0) skip_flag = *reinterpret_cast<volatile int*>(p.status);
   tc_fence_before_sync();
   __syncthreads();
@@ -220,11 +243,9 @@ __global__ void __launch_bounds__(640, 1)
     return;
   }
   volatile int* abort_p = &abort_flag;
-  const bool run = (abort_flag == 0) && (T_total > 0);
+  const bool run = (abort_flag == 0) && (plan.t_total > 0);
 
-  auto q_head = [&](int t) { return hkv * G + (t0 + t) / nI; };
-  auto q_tile = [&](int t) { return i_begin + (t0 + t) % nI; };
-
+  const int G = p.Hq / p.Hkv;
   // Register budget.  The launch gives every thread 96 registers (640 x 96 = 61440, the pool the warpgroups trade
   // inside); each role changes its own allowance on entry: 4 service warps x 64, 8 elementwise warps x 128,
   // 8 reduction warps x 80.  The raise waits until the other roles have lowered theirs, so the sum must fit the pool.
@@ -234,6 +255,8 @@ __global__ void __launch_bounds__(640, 1)
     if (warp == 0) {
       // =========================== TMA producer ===========================
       if (lane == 0 && run) {
+        const BwdWalk walk(plan, G);
+        const int hkv = plan.hkv, b = plan.b, hf = plan.hf, n0 = plan.kvt * 128, T_total = plan.t_total;
         tma_prefetch_desc(&tm_q);
         tma_prefetch_desc(&tm_k);
         tma_prefetch_desc(&tm_v);
@@ -269,8 +292,8 @@ __global__ void __launch_bounds__(640, 1)
           return true;
         };
         for (int t = 0; t < T_total; ++t) {
-          const int hq = q_head(t);
-          const int i = q_tile(t);
+          const int hq = walk.head(t);
+          const int i = walk.tile(t);
           // With as many dO slots as Q slots the dO slot frees first (after the dV product, the Q slot after dK); with fewer
           // the Q slot of tile t has been free since dK of tile t - 2.
           const bool ok = (NSO < NSQ) ? (load_q(t, hq, i) && load_do(t, hq, i)) : (load_do(t, hq, i) && load_q(t, hq, i));
@@ -282,6 +305,8 @@ __global__ void __launch_bounds__(640, 1)
       // =========================== MMA issuer ===========================
       // The whole warp runs the loop converged (cheap, warp-uniform descriptor arithmetic); the elected lane issues.
       if (run) {
+        const BwdWalk walk(plan, G);
+        const int hf = plan.hf, T_total = plan.t_total;
         const uint32_t el = elect_one();
         constexpr uint32_t idesc_s = make_idesc(128, BQ, kBf16, false, false);   // K-major x K-major
         // dV and dK (A from tensor memory / K-major, B MN-major) are as wide as the head dim, not as its padded size (head dim
@@ -358,25 +383,32 @@ __global__ void __launch_bounds__(640, 1)
             mma_ss_lo_e(tmem_base + Cfg::kTmDQ, k_mn + ((ks * 2048) >> 4), ds_mn + ((ks * 2048) >> 4), idesc_dq, ks > 0 ? 1u : 0u, el);
         };
 
-        // Padding rows of the operands that a product contracts over are cleared before its first use of them.
+        // Padding rows are cleared before the first product that reads them: those of K, Q and dO because a product contracts
+        // over them, those of V because dP of a padding key meets a weight of 0 (delta of a padding query is 0 as well).
+        const bool border_q = sc.has_mask && (plan.real_lo > sc.q_pos + plan.i_begin * BQ ||
+                                              plan.real_hi < sc.q_pos + (plan.i_begin + plan.n_i) * BQ);
         auto clear_tile = [&](uint32_t tile, int panels, int rows, int pos) {
-          if (real_lo > pos || real_hi < pos + rows) clear_padding_rows(tile, panels, rows, real_lo - pos, real_hi - pos, lane);
+          if (plan.real_lo > pos || plan.real_hi < pos + rows)
+            clear_padding_rows(tile, panels, rows, plan.real_lo - pos, plan.real_hi - pos, lane);
         };
         auto start_s = [&](int t, int st) {
           tc_fence_after_sync();
-          if (sc.has_mask) clear_tile(s_q + st * Cfg::kQBytes, Cfg::kPanels, BQ, sc.q_pos + q_tile(t) * BQ);
+          if (border_q) clear_tile(s_q + st * Cfg::kQBytes, Cfg::kPanels, BQ, sc.q_pos + walk.tile(t) * BQ);
           issue_s(st);
           mma_commit_e(&bar_s_full, el);
         };
         auto start_dp = [&](int t, int so) {
           tc_fence_after_sync();
-          if (sc.has_mask) clear_tile(s_do + so * Cfg::kQBytes, Cfg::kPanels, BQ, sc.q_pos + q_tile(t) * BQ);
+          if (border_q) clear_tile(s_do + so * Cfg::kQBytes, Cfg::kPanels, BQ, sc.q_pos + walk.tile(t) * BQ);
           issue_dp(so);
           mma_commit_e(&bar_dp_full, el);
         };
 
         bool ok = mbar_wait_warp(&bar_kv_full, 0, abort_p);
-        if (ok && sc.has_mask) clear_tile(s_k, Cfg::kKSmemBytes / kPanelK, 128, sc.k_pos + n0);
+        if (ok && sc.has_mask) {
+          clear_tile(s_k, Cfg::kKSmemBytes / kPanelK, 128, sc.k_pos + plan.kvt * 128);
+          clear_tile(s_v, Cfg::kPanels, 128, sc.k_pos + plan.kvt * 128);
+        }
         if (ok && Cfg::kKTmem) ok = mbar_wait_warp(&bar_k_tmem, 0, abort_p);
         if (ok) ok = mbar_wait_warp(&bar_q_full[0], 0, abort_p);
         if (ok) {
@@ -454,6 +486,9 @@ __global__ void __launch_bounds__(640, 1)
     const int cw = (warp - 4) >> 2;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;  // kv row inside the tile
+    const BwdWalk walk(plan, G);
+    const int b = plan.b, hkv = plan.hkv, hf = plan.hf, n0 = plan.kvt * 128, T_total = plan.t_total;
+    const int full_lo = plan.full_lo, full_hi = n0 + 128 > p.Skv ? INT_MIN : plan.full_hi;
     const int kvpos = n0 + row;
     // Queries of the block that see this key: [lo, lo + width).  Rows behind the block's end are seen by none.
     int lo = 0, width = 0;
@@ -478,7 +513,8 @@ __global__ void __launch_bounds__(640, 1)
     const int ahead = sc.q_pos + col0 - (sc.k_pos + kvpos);  // of query column col0 of tile 0 over this key
     bool ok = run;
     if (Cfg::kKTmem && run) {
-      // K (16 bit, two per column) into tensor memory: each thread copies half of its row from global memory, once per CTA
+      // K (16 bit, two per column) into tensor memory: each thread copies half of its row from global memory, once per CTA (zeros
+      // for a key that no query sees: padding, or behind the block's end)
       const T* krow = static_cast<const T*>(p.k) + ((static_cast<size_t>(b) * p.Skv + kvpos) * p.Hkv + hkv) * p.D;
 #pragma unroll 1
       for (int c = 0; c < DP / 4; c += 32) {
@@ -487,7 +523,7 @@ __global__ void __launch_bounds__(640, 1)
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           uint4 w = make_uint4(0, 0, 0, 0);
-          if (kvpos < p.Skv && col + k * 8 < p.D) w = *reinterpret_cast<const uint4*>(krow + col + k * 8);
+          if (width > 0 && col + k * 8 < p.D) w = *reinterpret_cast<const uint4*>(krow + col + k * 8);
           u[4 * k + 0] = w.x; u[4 * k + 1] = w.y; u[4 * k + 2] = w.z; u[4 * k + 3] = w.w;
         }
         tmem_st32(tmem_base + lane_addr + Cfg::kTmK + col / 2, u);
@@ -498,14 +534,14 @@ __global__ void __launch_bounds__(640, 1)
     }
     for (int t = 0; t < T_total && ok; ++t) {
       const int st = t % NSQ;
-      const int i = q_tile(t);
+      const int i = walk.tile(t);
       const float* lse2_s = reinterpret_cast<const float*>(stat_ptr + st * Cfg::kStatBytes) + col0;
       const float* delta_s = lse2_s + BQ;
       if (!mbar_wait_warp(&bar_q_full[st], (t / NSQ) & 1, abort_p)) { ok = false; break; }
       if (!mbar_wait_warp(&bar_s_full, t & 1, abort_p)) { ok = false; break; }
       tc_fence_after_sync();
       const int q0 = i * BQ + col0;
-      const bool masked = i * BQ < full_lo || i * BQ + BQ > full_hi || n0 + 128 > p.Skv;
+      const bool masked = i * BQ < full_lo || i * BQ + BQ > full_hi;
       uint32_t pk[NCH * 16];  // W = P (1 - tanh^2) for dX, in 16 bits like the P of the dV product
       {
         uint32_t r[NCH][32];
@@ -516,7 +552,7 @@ __global__ void __launch_bounds__(640, 1)
         for (int c = 1; c < NCH; ++c) reg_fence32(r[c]);
         // P^T = exp2(z - lse2) = exp2(-y); the distance term slope |i - j| is linear in the query where all queries of the
         // tile lie on one side of all keys.
-        const float slope = kKind > 0 ? slope_log2(sc, b, p.Hq, q_head(t)) : 0.f;
+        const float slope = kKind > 0 ? slope_log2(sc, b, p.Hq, walk.head(t)) : 0.f;
         const int d0 = sc.q_pos + i * BQ - (sc.k_pos + n0);  // of the first query over the first key
         const bool linear = d0 >= 127 || d0 + BQ - 1 <= 0 || slope == 0.f;
         const float sign_slope = d0 >= 127 ? slope : -slope;
@@ -605,13 +641,6 @@ __global__ void __launch_bounds__(640, 1)
                            sub2(pack_u2(r[c][4 * k + 0], r[c][4 * k + 1]), pack_f2(d4.x, d4.y))), s0, s1);
             unpack_f2(mul2(pack_f2(p23.x, p23.y),
                            sub2(pack_u2(r[c][4 * k + 2], r[c][4 * k + 3]), pack_f2(d4.z, d4.w))), s2, s3);
-            if (masked) {  // dP of a padding row may be anything
-              const int qp = q0 + c * 32 + k * 4 - lo;
-              if (static_cast<unsigned>(qp + 0) >= static_cast<unsigned>(width)) s0 = 0.f;
-              if (static_cast<unsigned>(qp + 1) >= static_cast<unsigned>(width)) s1 = 0.f;
-              if (static_cast<unsigned>(qp + 2) >= static_cast<unsigned>(width)) s2 = 0.f;
-              if (static_cast<unsigned>(qp + 3) >= static_cast<unsigned>(width)) s3 = 0.f;
-            }
             w[2 * k + 0] = Pack2<T>::pack(s0, s1);
             w[2 * k + 1] = Pack2<T>::pack(s2, s3);
           }
@@ -636,9 +665,9 @@ __global__ void __launch_bounds__(640, 1)
     // dK and dV are bit-reproducible too.  The run waited for has a lower block index: it was dispatched before.
     int* part_sem = nullptr;
     if (p.dq_order != nullptr && p.nsplit > 1) {
-      part_sem = p.dq_order + static_cast<size_t>(p.B) * p.Hq * nQtiles * Cfg::kHalves * 8 +
-                 (((static_cast<size_t>(b) * p.Hkv + hkv) * (nkvt) + kvt) * Cfg::kHalves + hf) * 8 + (warp - 4);
-      if ((ok || !run) && !wait_count(part_sem, part, lane == 0, abort_p)) ok = false;
+      part_sem = p.dq_order + static_cast<size_t>(p.B) * p.Hq * ((p.Sq + BQ - 1) / BQ) * Cfg::kHalves * 8 +
+                 (((static_cast<size_t>(b) * p.Hkv + hkv) * ((p.Skv + 127) / 128) + plan.kvt) * Cfg::kHalves + hf) * 8 + (warp - 4);
+      if ((ok || !run) && !wait_count(part_sem, plan.part, lane == 0, abort_p)) ok = false;
     }
     const bool unseen = T_total <= 0 && !p.reduce_out;  // no query sees any of these keys: zeros
     if (ok || unseen) {
@@ -708,6 +737,8 @@ __global__ void __launch_bounds__(640, 1)
     const int half = (warp - 12) >> 2;
     const int quarter = warp & 3;
     const int drow = quarter * 32 + lane;  // row of dQ^T = head-dim index inside this CTA's half
+    const BwdWalk walk(plan, G);
+    const int b = plan.b, hf = plan.hf, T_total = plan.t_total;
     const int d = hf * DH + drow;
     const bool d_ok = (drow < DH) && (hf * DH + quarter * 32 < p.D);  // the same for the whole warp
     // Warps with nothing but padding in their rows only take part in releasing the columns: in a loop of their own, except
@@ -729,8 +760,8 @@ __global__ void __launch_bounds__(640, 1)
     const int nQt128 = p.Spad / 128;
     bool ok = run && (!kApart || d_ok);
     for (int t = 0; t < T_total && ok; ++t) {
-      const int hq = q_head(t);
-      const int q0 = q_tile(t) * BQ;
+      const int hq = walk.head(t);
+      const int q0 = walk.tile(t) * BQ;
       if (!mbar_wait_warp(&bar_dq_full, t & 1, abort_p)) { ok = false; break; }
       tc_fence_after_sync();
       float* base = p.dq_acc + ((static_cast<size_t>(b) * p.Hq + hq) * nQt128 + q0 / 128) * kTileElems +
@@ -753,9 +784,9 @@ __global__ void __launch_bounds__(640, 1)
       int* order_sem = nullptr;
       if (p.dq_order != nullptr) {
         order_sem = p.dq_order +
-                    ((((static_cast<size_t>(b) * p.Hq + hq) * nQtiles + q_tile(t)) * Cfg::kHalves + hf) * 2 + half) * 4 +
+                    ((((static_cast<size_t>(b) * p.Hq + hq) * ((p.Sq + BQ - 1) / BQ) + q0 / BQ) * Cfg::kHalves + hf) * 2 + half) * 4 +
                     quarter;
-        if (!wait_count(order_sem, kvt, lane == 0 && d_ok, abort_p)) { ok = false; break; }
+        if (!wait_count(order_sem, plan.kvt, lane == 0 && d_ok, abort_p)) { ok = false; break; }
       }
       if (!kApart && !d_ok) continue;
       if (Cfg::kStageDQ && order_sem == nullptr) {
