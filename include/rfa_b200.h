@@ -239,7 +239,7 @@ int rfa_bwd_local(const void* q, const void* k, const void* v, const void* out, 
  */
 typedef struct rfa_score_args {
   float softmax_scale;      /* > 0 */
-  float softcap;            /* > 0: cap of the scores; 0: none */
+  float softcap;            /* up to 1000: cap of the scores; 0: none */
   const float* slopes;      /* NULL, or distance slopes (>= 0 or < 0): [Hq], or [B, Hq] with slopes_per_batch */
   int slopes_per_batch;
   int causal;               /* without a mask: key j is seen by query i when j <= i; with one: as the mask was built */

@@ -765,12 +765,13 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
           for (int g = 0; g < NG; ++g) {
             sc0[g] = Kv4Type<T>::lo(e0[g]);
             sc1[g] = Kv4Type<T>::lo(e1[g]);
-            most = max3_nan(most, sc0[g], sc1[g]);
+            most = fmaxf(fmaxf(most, sc0[g]), sc1[g]);
           }
-          if (__any_sync(0xffffffffu, !(most <= v_limit))) {
+          if (__any_sync(0xffffffffu, most > v_limit && most < INFINITY)) {
             // the first scales, or 2^8 above those the power was chosen for: it is chosen again, the largest comes to [1, 2)
+            if (!(most < INFINITY)) most = 0.f;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
+            for (int d = 1; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
             const int ex = min(max(static_cast<int>(__float_as_uint(most) >> 23), 10), 245);
             const float down = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
             const float f = down / v_down;
@@ -1122,7 +1123,7 @@ extern "C" int rfa_kv4_attn(const void* q, const long long* q_strides, const voi
   const int rc = kv4_check(codes, meta, n_pages, table, max_pages, lens, B, T, Hkv, D, dtype);
   if (rc != RFA_OK) return rc;
   if (Hq <= 0 || Hq % Hkv != 0) return RFA_ERR_INVALID_ARG;
-  if (!(softmax_scale > 0.f) || !(softmax_scale <= 3.0e38f) || !(softcap >= 0.f) || !(softcap <= 3.0e38f))
+  if (!(softmax_scale > 0.f) || !(softmax_scale <= 3.0e38f) || !(softcap >= 0.f) || !(softcap <= kMaxCap))
     return RFA_ERR_INVALID_ARG;
   for (int i = 0; i < 3; ++i)
     if (q_strides[i] % 8 != 0) return RFA_ERR_INVALID_ARG;

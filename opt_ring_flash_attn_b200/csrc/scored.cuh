@@ -14,6 +14,8 @@
 namespace rfa {
 
 constexpr float kLog2e = 1.4426950408889634f;
+// Largest cap: cap * tanh comes out of cap - 2 cap / (exp + 1) with an error of 2^-24 cap, 6e-5 of a weight here.
+constexpr float kMaxCap = 1000.f;
 // Running maximum of a row that has seen no key: finite, so that exp2(-inf - kNoKey) is 0 and not NaN, and far below any
 // score in log2 units that could matter, so that the first real one rescales what was there by 0.
 constexpr float kNoKey = -1e30f;
@@ -76,7 +78,7 @@ struct ScoreParams {
 // Checks and unpacks the arguments of an entry point.
 inline int make_score_params(const rfa_score_args* a, int B, int S, ScoreParams* out) {
   if (!a || !(a->softmax_scale > 0.f) || !(a->softcap >= 0.f)) return RFA_ERR_INVALID_ARG;
-  if (!(a->softmax_scale <= 3.0e38f) || !(a->softcap <= 3.0e38f)) return RFA_ERR_INVALID_ARG;
+  if (!(a->softmax_scale <= 3.0e38f) || !(a->softcap <= kMaxCap)) return RFA_ERR_INVALID_ARG;
   if (a->shards < 1 || a->q_shard < 0 || a->q_shard >= a->shards || a->k_shard < 0 || a->k_shard >= a->shards)
     return RFA_ERR_INVALID_ARG;
   if (static_cast<long long>(S) * a->shards > INT_MAX / 2) return RFA_ERR_TOO_LARGE;

@@ -24,6 +24,9 @@ from . import _native, schedule, workspace
 from .api import _deterministic_now, _validate
 
 
+MAX_SOFTCAP = 1000.0  # above, the tanh would lose too much in fp32
+
+
 class DocumentMask:
     """Which keys the queries of a batch see (made by :func:`document_mask`).  It lives on the device; the forward and the
     backward passes of every layer that works on the same batch read it."""
@@ -239,8 +242,8 @@ def _check_slopes(slopes: Optional[torch.Tensor], B: int, Hq: int, device: torch
 
 def _check_softcap(softcap: float) -> float:
     softcap = float(softcap or 0.0)
-    if not (softcap >= 0.0) or math.isinf(softcap):
-        raise ValueError(f"softcap must be 0 (none) or a positive number, got {softcap}")
+    if not (0.0 <= softcap <= MAX_SOFTCAP):
+        raise ValueError(f"softcap must be 0 (none) or a positive number up to {MAX_SOFTCAP:g}, got {softcap}")
     return softcap
 
 
@@ -283,7 +286,7 @@ def scored_flash_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax
 
     Args:
       q, k, v, softmax_scale, causal, group: as in :func:`ring_flash_attn`.
-      softcap: scores are capped to ``softcap * tanh(score / softcap)``; 0 leaves them as they are.
+      softcap: scores are capped to ``softcap * tanh(score / softcap)``, softcap up to 1000; 0 leaves them as they are.
       alibi_slopes: fp32 ``[H_q]`` or ``[B, H_q]``; ``slope * |i - j|`` is taken off the (capped) score.  Not differentiable.
       mask: documents and prefixes, from :func:`document_mask` with the same ``causal`` and ``group``.
 

@@ -6,8 +6,15 @@ The bounds count roundings.  With u = finfo(dtype).eps / 2 (half a step of the 1
   dQ   W = P (1 - tanh^2) and dX are rounded (2 u |dX|), delta = sum(dO o out) is formed from the rounded out, off by
        D_i = |dO_i| . u (A_i + |out_i|), so dX is off by 2 u |dX| + W D; times |K| and the scale, and the result's rounding;
   dK   the same, times |Q|.
-EXTRA covers the arithmetic in fp32 between the roundings: exp2 to 2^-22 and the quartic to 2^-17, scores summed over up to
-256 products (2^-24 sqrt(256) of |q||k| scale < 40: 4e-5), tanh to 2^-22 of a cap of at most 50 (1e-5), all relative to P.
+Rounding to fp16 is off by u of the value or, below its smallest normal number, by half its smallest step, h = 2^-25 (bf16
+reaches down to 2^-133): P adds h sum|V| and h sum|dO|, W adds h |dP - delta|, dX adds h.
+EXTRA covers the arithmetic in fp32 between the roundings: exp2 to 2^-22 and the quartic to 2^-17, tanh to 2^-22 of a cap of at
+most 50 (1e-5; a larger cap C adds C 2^-22), all relative to P.
+The scores themselves: products of 16-bit numbers are exact in fp32, their sum over the head dim is taken in steps of 16, each
+off by at most 2^-23 of the magnitudes so far: e_x = (D / 16 + 2) 2^-23 scale |q|.|k|.  Behind the cap that is e_y = (1 -
+tanh^2) e_x, which moves a weight by e_y and its row's sum by sum(P e_y), relative to P; 1 - tanh^2 itself moves by 2 e_x / cap
+of its value (its derivative is -2 tanh (1 - tanh^2) / cap).  Large scores feel this (|q||k| scale = 1e5: e_x = 0.07), ordinary
+ones do not (30: 2e-5).
 """
 import math
 
@@ -34,6 +41,7 @@ def reference(q, k, v, dout, vis, *, causal_pos=None, scale=None, softcap=0.0, s
     B, S, Hq, D = q.shape
     G = Hq // k.shape[2]
     u = torch.finfo(q.dtype).eps / 2
+    h2 = torch.finfo(q.dtype).smallest_normal * u  # half the smallest step
     scale = D ** -0.5 if scale is None else scale
     pos = torch.arange(S, device=q.device, dtype=torch.float64)
     names = ("out", "dq", "dk", "dv")
@@ -51,8 +59,10 @@ def reference(q, k, v, dout, vis, *, causal_pos=None, scale=None, softcap=0.0, s
             K = k[b, :, h // G].double().masked_fill(~cols[:, None], 0)
             V = v[b, :, h // G].double().masked_fill(~cols[:, None], 0)
             x = Q @ K.T * scale
-            jac = torch.ones_like(x)
+            jac, jac_off = torch.ones_like(x), torch.zeros_like(x)
+            e_x = (D / 16 + 2) * 2.0 ** -23 * (Q.abs() @ K.abs().T) * scale
             if softcap:
+                jac_off = 2 * e_x / softcap
                 t = torch.tanh(x / softcap)
                 x, jac = softcap * t, 1 - t * t
             if slopes is not None:
@@ -62,21 +72,24 @@ def reference(q, k, v, dout, vis, *, causal_pos=None, scale=None, softcap=0.0, s
             lse[b, h] = torch.logsumexp(x, 1)
             P = torch.exp(x - lse[b, h][:, None]).masked_fill(~seen, 0)
             O, A = P @ V, P @ V.abs()
+            e_y = jac * e_x + softcap * 2.0 ** -22
+            e_p = EXTRA + e_y + (P * e_y).sum(1, keepdim=True)  # of a weight, relative
+            E = (P * e_p + h2 * seen) @ V.abs()
             val["out"][b, :, h] = O
-            err["out"][b, :, h] = (u + EXTRA) * A + u * O.abs()
+            err["out"][b, :, h] = u * A + E + u * O.abs()
             dP = dO @ V.T
             delta = (dO * O).sum(1)
             W = P * jac
             dX = W * (dP - delta[:, None])
-            off = (dO.abs() * (u * (A + O.abs()) + EXTRA * A)).sum(1)
+            off = (dO.abs() * (u * (A + O.abs()) + E)).sum(1)
             # fp32 relative errors act on both terms of the difference
-            dX_err = 2 * u * dX.abs() + W * off[:, None] + EXTRA * W * ((dO.abs() @ V.abs().T) + delta.abs()[:, None])
+            dX_err = h2 * seen * (1 + (dP - delta[:, None]).abs()) + 2 * u * dX.abs() + W * off[:, None] + (e_p + jac_off) * W * ((dO.abs() @ V.abs().T) + delta.abs()[:, None])
             val["dq"][b, :, h] = dX @ K * scale
             err["dq"][b, :, h] = dX_err @ K.abs() * scale
             val["dk"][b, :, h // G] += dX.T @ Q * scale
             err["dk"][b, :, h // G] += dX_err.T @ Q.abs() * scale
             val["dv"][b, :, h // G] += P.T @ dO
-            err["dv"][b, :, h // G] += (u + EXTRA) * (P.T @ dO.abs())
+            err["dv"][b, :, h // G] += (P * (u + e_p) + h2 * seen).T @ dO.abs()
     for n in ("dq", "dk", "dv"):
         err[n] += u * val[n].abs()
     # 1e-6: fp16 results below its smallest normal number are rounded to multiples of 2^-24

@@ -217,6 +217,37 @@ def test_peaked_weights(peak):
     _check(out, lse, attn_reference(q, values, [n]))
 
 
+def test_scales_far_apart():
+    """V of very different sizes from token to token (the power of two that keeps P sc in fp16 is chosen again on the way), and
+    a V that is no number, which reaches its own 32 channels only."""
+    import opt_ring_flash_attn_b200 as rfa
+
+    for dt, top in ((BF, 1e20), (HF, 2e3)):
+        n = 1000
+        table, pool = _table([n])
+        cache = rfa.KV4Cache.empty(pool, 1, 128, dt, DEV)
+        k = torch.randn(1, n, 1, 128, generator=_gen(1), device=DEV).to(dt)
+        v = torch.randn(1, n, 1, 128, generator=_gen(2), device=DEV)
+        v[0, :300] /= top
+        v[0, 300:310] = 0
+        v[0, 500:] *= top / 10
+        v = v.to(dt)
+        rfa.kv4_append(cache, k, v, table, _ints([0]))
+        values = [(quantized(k[0]), quantized(v[0]))]
+        q = torch.randn(1, 1, 4, 128, generator=_gen(3), device=DEV).to(dt)
+        for m in (n, 700, 310, 305, 5):
+            ref = attn_reference(q, [(values[0][0][:m], values[0][1][:m])], [m])
+            out, lse = rfa.kv4_attn_with_lse(q, cache, table, _ints([m]))
+            _check(out, lse, (ref[0], ref[1] * (1 + 1e-6), ref[2]))
+        v[0, 400, 0, 40] = math.nan
+        rfa.kv4_append(cache, k, v, table, _ints([0]))
+        ref = attn_reference(q, values, [n])
+        out, lse = rfa.kv4_attn_with_lse(q, cache, table, _ints([n]))
+        assert out[..., 32:64].isnan().all()
+        keep = [c for c in range(128) if not 32 <= c < 64]
+        _check(out[..., keep], lse, (ref[0][..., keep], ref[1][..., keep], ref[2]))
+
+
 def test_bad_pages_and_lengths():
     """A table entry outside the pool: its tokens do not exist.  Lengths beyond the table end at it; negative ones are zero."""
     import opt_ring_flash_attn_b200 as rfa

@@ -105,12 +105,25 @@ def test_documents_per_row(D, dt, deterministic):
         assert all(torch.equal(got[n], again[n]) for n in got)
 
 
-@pytest.mark.parametrize("value", [1e-3, 1.0, 1e4])
-def test_cap_over_its_whole_range(value):
-    """Scores far below the cap, around it and far beyond it (where tanh is 1 and nothing flows back)."""
-    q, k, v, dout = inputs(4, 1, 200, 2, 2, 64, BF, DEV, std=math.sqrt(value))
-    ref = reference(q, k, v, dout, visible(200, True, device=DEV), softcap=5.0)
-    check(ref, **_run(q, k, v, dout, causal=True, softcap=5.0))
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("value,cap", [(1e-3, 5.0), (0.6, 5.0), (1.0, 5.0), (4.0, 5.0), (1e4, 5.0), (1.0, 1000.0), (4.0, 0.01)])
+def test_cap_over_its_whole_range(D, value, cap):
+    """Scores far below the cap, around it (where one route to the tanh hands over to the other) and far beyond it (where it
+    is 1 and nothing flows back); the largest cap and a tiny one."""
+    q, k, v, dout = inputs(4, 1, 700, 2, 2, D, HF, DEV, std=math.sqrt(value))
+    ref = reference(q, k, v, dout, visible(700, True, device=DEV), softcap=cap)
+    check(ref, **_run(q, k, v, dout, causal=True, softcap=cap))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_outliers_beyond_the_cap(D):
+    """A few scores beyond the cap among ordinary ones, at the start, inside and at the end of a tile, in one head of two."""
+    S = 520
+    q, k, v, dout = inputs(15, 1, S, 2, 1, D, BF, DEV)
+    q[0, [5, 200, 519], 1] *= 30
+    k[0, [0, 127, 128, 300], 0] *= 20
+    ref = reference(q, k, v, dout, visible(S, True, device=DEV), softcap=15.0)
+    check(ref, **_run(q, k, v, dout, causal=True, softcap=15.0))
 
 
 def test_gradient_against_differences():

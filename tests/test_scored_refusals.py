@@ -13,6 +13,7 @@ def _qkv(B=1, S=16, H=2, D=64):
 @pytest.mark.parametrize("kw,message", [
     (dict(softcap=-1.0), "softcap"),
     (dict(softcap=float("inf")), "softcap"),
+    (dict(softcap=1001.0), "softcap"),
     (dict(softcap=float("nan")), "softcap"),
     (dict(softmax_scale=0.0), "softmax_scale"),
     (dict(softmax_scale=float("inf")), "softmax_scale"),
@@ -80,6 +81,7 @@ def test_abi_refuses_bad_arguments():
     assert fwd(None) == -1
     assert fwd(args(softmax_scale=0.0)) == -1
     assert fwd(args(softcap=-1.0)) == -1
+    assert fwd(args(softcap=2000.0)) == -1
     assert fwd(args(softcap=float("nan"))) == -1
     assert fwd(args(shards=2, q_shard=2)) == -1
     assert fwd(args(shards=0)) == -1
