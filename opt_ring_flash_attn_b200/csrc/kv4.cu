@@ -82,6 +82,10 @@ __device__ __noinline__ float border_code(float x, float lo, float sc, float t) 
   return fminf(up ? below + 1.f : below, 15.f);
 }
 
+// Scales below the smallest normal number of their type keep fewer bits, and 15 of them may fall short of the range.
+template <typename T>
+constexpr float kSmallScale = Pack2<T>::kIsBf16 ? 1.1754944e-38f * 18446744073709551616.f : 6.103515625e-5f;
+
 // Codes of 8 channels (one lane), low bits first, and the group's (sc, min) in T's bits.
 template <typename T>
 __device__ __forceinline__ uint32_t quantize8(const uint4& raw, uint32_t& meta) {
@@ -95,10 +99,14 @@ __device__ __forceinline__ uint32_t quantize8(const uint4& raw, uint32_t& meta) 
   ends = max2_nan<T>(ends, __shfl_xor_sync(0xffffffffu, ends, 2));
   const float hi = Kv4Type<T>::lo(ends);
   float lo = -Kv4Type<T>::hi(ends);
-  const uint16_t sb = Kv4Type<T>::bits((hi - lo) / 15.f);
+  // (hi - lo) / 15, correctly rounded: the quotient with a rounded reciprocal, put right by its exact remainder
+  const float span = hi - lo;
+  const float q = span * 0.06666667f;
+  const uint16_t sb = Kv4Type<T>::bits(span < INFINITY ? fmaf(fmaf(-15.f, q, span), 0.06666667f, q) : span);
   float sc = Kv4Type<T>::value(sb);
   meta = static_cast<uint32_t>(sb) | ((ends ^ sign) & 0xffff0000u);
   if (!(sc > 0.f)) return 0;
+  // channels i and i + 4 as a pair
   float x[8] = {Kv4Type<T>::lo(raw.x), Kv4Type<T>::hi(raw.x), Kv4Type<T>::lo(raw.y), Kv4Type<T>::hi(raw.y),
                 Kv4Type<T>::lo(raw.z), Kv4Type<T>::hi(raw.z), Kv4Type<T>::lo(raw.w), Kv4Type<T>::hi(raw.w)};
   if (sc < 1e-30f) {  // its reciprocal would leave fp32 (bf16 only): the same codes under a power of two
@@ -108,27 +116,36 @@ __device__ __forceinline__ uint32_t quantize8(const uint4& raw, uint32_t& meta) 
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] *= up;
   }
-  // (x - lo) * (1 / sc) is off by less than 3e-6 in 15, so its nearest whole number is the code unless it lies within 1e-5
-  // of a border between two codes.
-  const float inv = 1.f / sc;
+  // (x - lo) * (1 / sc) is off by less than 6e-6 in 15, so its nearest whole number is the code unless it lies within 1e-5
+  // of a border between two codes, or beyond 15 because a small scale lost bits.
+  const float inv = fast_rcp(sc);
+  const uint64_t inv2 = pack_f2(inv, inv), lo2 = pack_f2(lo, lo);
   constexpr float magic = 12582912.f;  // 1.5 * 2^23: adding it rounds to a whole number, ties to even
+  const uint64_t magic2 = pack_f2(magic, magic);
   float u[8], away = 0.f;
+  uint64_t four = 0;  // four codes each, as numbers of 16 bits
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = fminf((x[i] - lo) * inv, 15.f);
-    u[i] = (t + magic) - magic;
-    away = fmaxf(away, fabsf(t - u[i]));
+  for (int i = 3; i >= 0; --i) {
+    const uint64_t t = mul2(sub2(pack_f2(x[i], x[i + 4]), lo2), inv2);
+    const uint64_t w = sub2(add2(t, magic2), magic2);
+    float a0, a1;
+    unpack_f2(sub2(t, w), a0, a1);
+    away = fmaxf(away, fmaxf(fabsf(a0), fabsf(a1)));
+    unpack_f2(w, u[i], u[i + 4]);
+    four = fma2(four, pack_f2(16.f, 16.f), w);
   }
-  if (away > 0.49999f) {
+  float p0, p1;
+  unpack_f2(four, p0, p1);
+  if (away > 0.49999f || sc < kSmallScale<T>) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float t = fminf((x[i] - lo) * inv, 15.f);
+      const float t = (x[i] - lo) * inv;
       if (fabsf(t - u[i]) > 0.49999f) u[i] = border_code(x[i], lo, sc, t);
+      u[i] = fminf(u[i], 15.f);
     }
+    p0 = fmaf(fmaf(fmaf(u[3], 16.f, u[2]), 16.f, u[1]), 16.f, u[0]);
+    p1 = fmaf(fmaf(fmaf(u[7], 16.f, u[6]), 16.f, u[5]), 16.f, u[4]);
   }
-  // four codes each, as a number of 16 bits
-  const float p0 = fmaf(fmaf(fmaf(u[3], 16.f, u[2]), 16.f, u[1]), 16.f, u[0]);
-  const float p1 = fmaf(fmaf(fmaf(u[7], 16.f, u[6]), 16.f, u[5]), 16.f, u[4]);
   return static_cast<uint32_t>(__float2int_rn(p0)) | (static_cast<uint32_t>(__float2int_rn(p1)) << 16);
 }
 
