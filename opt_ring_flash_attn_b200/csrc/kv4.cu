@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(T* __restrict__ k, T* _
 // A code in bits 0-3 or 4-7 of a half word read as fp16 is u 2^-24 or u 2^-20 (subnormal numbers, which the products take as
 // they are), so one logic operation takes two codes out and two of four need no shift.  (The same nibble as an e4m3 byte is
 // u 2^-9, one operation for four codes, but products of e4m3 are widened to fp16 on the same logic unit: 57 million
-// instructions instead of XX.)
+// instructions instead of 42.)
 //   q enters as fp16, each row under a power of two and the channels of odd codes under 2^-4 of it: exact for fp16 and bf16.
 //   The minima meet the group sums of q, split in two 16-bit parts, in one more product with the meta words as they are.
 //   P sc is rounded to fp16 (11 bits, for bf16 caches too), under a power of two that keeps it in range.  For fp16 results
@@ -470,11 +470,16 @@ struct Kv4Cfg {
   static_assert(kBlocksPerSm * (kSmemBytes + 1024 + 256) <= 228 * 1024, "shared memory over budget");
 };
 
-template <typename T, int NG, int NT>
+template <typename T, int NG, int NT, bool kHalf>
 __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_kernel(const Kv4AttnParams p) {
   using Cfg = Kv4Cfg<NG, NT>;
   constexpr int kRing = Cfg::kRing, kRows = Cfg::kRows, D = Cfg::kD;
   constexpr bool kCentred = !Pack2<T>::kIsBf16;
+  // With four query rows or fewer, columns 0-3 are the rows over the first 16 of a warp's 32 tokens and columns 4-7 the same
+  // rows over the others (kSets token sets per S tile): half the work from the scores to P, and a sum of two at the end.
+  static_assert(!kHalf || NT == 1, "half columns are for one column tile");
+  constexpr int kJ = kHalf ? 1 : 2;               // S tiles of 16 tokens that are held apart
+  constexpr int kUsedRows = kHalf ? 4 : kRows;
   constexpr int kQuads = (NG + 3) / 4;
   constexpr float q_down = 1.f / 16777216.f;  // codes are u 2^-24
   extern __shared__ __align__(128) uint8_t smem[];
@@ -547,6 +552,8 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
   const int r = lane >> 2, c = lane & 3;  // S row / O row group, and column pair
   // S row r is token rt of each 8: V's loads then take tokens 0, 3, 4, 7 at a time, which lie in different banks by twos.
   const int rt = r ^ ((r >> 1) & 1);
+  const int far = kHalf ? (c >> 1) * 16 : 0;           // of this lane's tokens in S
+  const uint32_t first_set = r < 4 ? 0xffffffffu : 0;  // kHalf: columns (rows of the B operand's lanes) of the first set
   const int G = p.Hq / p.Hkv;
   const int n_rows = p.T * G;
   int n = 0;  // pages of the pair so far
@@ -563,7 +570,7 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
     int lim[NT][2];  // last key that the row sees
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = row0 + nt * 8 + r;
+      const int row = row0 + nt * 8 + (kHalf ? r & 3 : r);
       const T* src = static_cast<const T*>(p.q) + at.b * p.q_b + (row / G) * p.q_t + (head * G + row % G) * p.q_h + c * 8;
       uint4 x[NG];
       float top = 0.f;
@@ -608,7 +615,7 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
       const float back = ex == 255 ? __uint_as_float(0x7fc00000u) : 1.f / (up * q_down);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int col = row0 + nt * 8 + 2 * c + i;
+        const int col = row0 + nt * 8 + (kHalf ? (2 * c + i) & 3 : 2 * c + i);
         zs[nt][i] = __shfl_sync(0xffffffffu, back, (2 * c + i) * 4) * (p.cap_log2 > 0.f ? p.cap_in : p.scale_log2);
         lim[nt][i] = col < n_rows ? at.len - p.T + col / G : -1;
         slope[nt][i] = 0.f;
@@ -645,9 +652,10 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
         const uint8_t* kc = stage + (side * 32 + rt) * (D / 2) + c * NG * 4;
         const uint8_t* km = stage + Cfg::kCodeBytes + (side * 32 + rt) * (NG * 4);
         // ---- S, tokens pos0 + 16 j + r and + 8 ----
-        float s[2][NT][4];
+        float s[kJ][NT][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
+          float sj[NT][4];
           uint32_t w0[NG], w1[NG], e0[NG], e1[NG];
           lds_words<NG>(w0, kc + j * 16 * (D / 2));
           lds_words<NG>(w1, kc + (j * 16 + 8) * (D / 2));
@@ -656,7 +664,7 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) s[j][nt][x] = 0.f;
+            for (int x = 0; x < 4; ++x) sj[nt][x] = 0.f;
 #pragma unroll
           for (int k = 0; k < kQuads; ++k) {
             const bool any = k * 4 + c < NG;
@@ -664,7 +672,7 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
             const uint32_t b = any ? *reinterpret_cast<const uint32_t*>(km + (j * 16 + 8) * (NG * 4) + (k * 4 + c) * 4) : 0;
             const uint32_t mw[4] = {a, b, a, b};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816<T>(s[j][nt], mw, qs[nt][k][0], qs[nt][k][1]);
+            for (int nt = 0; nt < NT; ++nt) mma16816<T>(sj[nt], mw, qs[nt][k][0], qs[nt][k][1]);
           }
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
@@ -676,17 +684,24 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
               float acc[4] = {0.f, 0.f, 0.f, 0.f};
               mma16816<__half>(acc, a0, qf[nt][g][0], qf[nt][g][1]);
               mma16816<__half>(acc, a1, qf[nt][g][2], qf[nt][g][3]);
-              s[j][nt][0] = fmaf(acc[0], sc0, s[j][nt][0]);
-              s[j][nt][1] = fmaf(acc[1], sc0, s[j][nt][1]);
-              s[j][nt][2] = fmaf(acc[2], sc1, s[j][nt][2]);
-              s[j][nt][3] = fmaf(acc[3], sc1, s[j][nt][3]);
+              sj[nt][0] = fmaf(acc[0], sc0, sj[nt][0]);
+              sj[nt][1] = fmaf(acc[1], sc0, sj[nt][1]);
+              sj[nt][2] = fmaf(acc[2], sc1, sj[nt][2]);
+              sj[nt][3] = fmaf(acc[3], sc1, sj[nt][3]);
             }
           }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              if (kHalf) s[0][nt][x] = j == 0 || c < 2 ? (j == 0 ? sj[nt][x] : s[0][nt][x]) : sj[nt][x];
+              else s[j][nt][x] = sj[nt][x];
+            }
         }
         // ---- scores in log2 units, masks ----
         if (p.cap_log2 > 0.f) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < kJ; ++j)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -694,7 +709,7 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
                 s[j][nt][x] = fmaf(-2.f * p.cap_log2, fast_rcp(fast_exp2(s[j][nt][x] * zs[nt][x & 1]) + 1.f), p.cap_log2);
         } else {
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < kJ; ++j)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -705,9 +720,9 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const float ahead = static_cast<float>(lim[nt][x] - (pos0 + rt));  // of the row over its first key here
+              const float ahead = static_cast<float>(lim[nt][x] - (pos0 + far + rt));  // of the row over its first key here
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
+              for (int j = 0; j < kJ; ++j) {
                 s[j][nt][x] = fmaf(-slope[nt][x], ahead - 16.f * j, s[j][nt][x]);
                 s[j][nt][x + 2] = fmaf(-slope[nt][x], ahead - (16.f * j + 8.f), s[j][nt][x + 2]);
               }
@@ -715,12 +730,12 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
         }
         if (pos0 + 31 > at.len - p.T) {  // some row does not see all of them
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < kJ; ++j)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int x = 0; x < 4; ++x)
-                if (pos0 + j * 16 + rt + (x < 2 ? 0 : 8) > lim[nt][x & 1]) s[j][nt][x] = -INFINITY;
+                if (pos0 + far + j * 16 + rt + (x < 2 ? 0 : 8) > lim[nt][x & 1]) s[j][nt][x] = -INFINITY;
         }
         // ---- running maximum: it follows when a score is more than 2^2 above it, or is no number ----
         bool grow = false;
@@ -728,7 +743,8 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const float hi = max_nan(max3_nan(s[0][nt][x], s[0][nt][x + 2], s[1][nt][x]), s[1][nt][x + 2]);
+            float hi = max_nan(s[0][nt][x], s[0][nt][x + 2]);
+            if (!kHalf) hi = max3_nan(hi, s[kJ - 1][nt][x], s[kJ - 1][nt][x + 2]);
             grow = grow || !(hi - m[nt][x] <= 2.f);
           }
         if (__any_sync(0xffffffffu, grow)) {
@@ -736,7 +752,8 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              float top = max3_nan(m[nt][x], max_nan(s[0][nt][x], s[0][nt][x + 2]), max_nan(s[1][nt][x], s[1][nt][x + 2]));
+              float top = max3_nan(m[nt][x], s[0][nt][x], s[0][nt][x + 2]);
+              if (!kHalf) top = max3_nan(top, s[kJ - 1][nt][x], s[kJ - 1][nt][x + 2]);
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
               const float alpha = fast_exp2(m[nt][x] - top);
@@ -753,7 +770,7 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
             }
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < kJ; ++j)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -763,18 +780,16 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
             }
         // ---- O ----
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint8_t* vc = stage + kPage * (D / 2) + (side * 32 + j * 16 + 2 * c + (c & 1)) * (D / 2) + r * NG * 2;
-          const int v_next = (c & 1) ? -(D / 2) : D / 2;  // to the odd one of the two tokens
-          const uint8_t* vm = km + (kPage + j * 16) * (NG * 4);
+        for (int j = 0; j < kJ; ++j) {
+          const uint8_t* vm = km + (kPage + far + j * 16) * (NG * 4);
           uint32_t e0[NG], e1[NG];
           lds_words<NG>(e0, vm);
           lds_words<NG>(e1, vm + 8 * (NG * 4));
           if (there < 32) {  // tokens behind the last: their scales may be anything
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-              if (j * 16 + rt >= there) e0[g] = 0;
-              if (j * 16 + rt + 8 >= there) e1[g] = 0;
+              if (far + j * 16 + rt >= there) e0[g] = 0;
+              if (far + j * 16 + rt + 8 >= there) e1[g] = 0;
             }
           }
           float sc0[NG], sc1[NG], most = 0.f;
@@ -809,17 +824,10 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 4; ++x) pd[nt][x] = s[j][nt][x] * v_down;
-          uint32_t t0[(NG + 1) / 2], t1[(NG + 1) / 2], t8[(NG + 1) / 2], t9[(NG + 1) / 2];
-          lds_halves<NG>(t0, vc);
-          lds_halves<NG>(t1, vc + v_next);
-          lds_halves<NG>(t8, vc + 8 * (D / 2));
-          lds_halves<NG>(t9, vc + 8 * (D / 2) + v_next);
+          // P sc as the B operand, in fp16
+          uint32_t pb[NT][NG][2];
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            const uint32_t lo = __byte_perm(t0[g / 2], t1[g / 2], g % 2 ? 0x7632 : 0x5410);
-            const uint32_t hi = __byte_perm(t8[g / 2], t9[g / 2], g % 2 ? 0x7632 : 0x5410);
-            const uint32_t a0[4] = {codes_fp16<kCentred, 0>(lo), codes_fp16<kCentred, 1>(lo), codes_fp16<kCentred, 0>(hi), codes_fp16<kCentred, 1>(hi)};
-            const uint32_t a1[4] = {codes_fp16<kCentred, 2>(lo), codes_fp16<kCentred, 3>(lo), codes_fp16<kCentred, 2>(hi), codes_fp16<kCentred, 3>(hi)};
             float mn0 = Kv4Type<T>::hi(e0[g]), mn1 = Kv4Type<T>::hi(e1[g]);
             if (kCentred) {
               mn0 = fmaf(8.f, sc0[g], mn0);
@@ -827,12 +835,34 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              const uint32_t b0 = transpose8x8(Pack2<__half>::pack(pd[nt][0] * sc0[g], pd[nt][1] * sc0[g]));
-              const uint32_t b1 = transpose8x8(Pack2<__half>::pack(pd[nt][2] * sc1[g], pd[nt][3] * sc1[g]));
+              pb[nt][g][0] = transpose8x8(Pack2<__half>::pack(pd[nt][0] * sc0[g], pd[nt][1] * sc0[g]));
+              pb[nt][g][1] = transpose8x8(Pack2<__half>::pack(pd[nt][2] * sc1[g], pd[nt][3] * sc1[g]));
               corr[nt][g][0] = fmaf(s[j][nt][0], mn0, fmaf(s[j][nt][2], mn1, corr[nt][g][0]));
               corr[nt][g][1] = fmaf(s[j][nt][1], mn0, fmaf(s[j][nt][3], mn1, corr[nt][g][1]));
-              mma16816<__half>(o[nt][g][0], a0, b0, b1);
-              mma16816<__half>(o[nt][g][1], a1, b0, b1);
+            }
+          }
+#pragma unroll
+          for (int set = 0; set < 3 - kJ; ++set) {  // kHalf: both token sets, each with its columns of P
+            const uint8_t* vc = stage + kPage * (D / 2) + (side * 32 + (j + set) * 16 + 2 * c + (c & 1)) * (D / 2) + r * NG * 2;
+            const int v_next = (c & 1) ? -(D / 2) : D / 2;  // to the odd one of the two tokens
+            const uint32_t keep = set == 0 ? first_set : ~first_set;
+            uint32_t t0[(NG + 1) / 2], t1[(NG + 1) / 2], t8[(NG + 1) / 2], t9[(NG + 1) / 2];
+            lds_halves<NG>(t0, vc);
+            lds_halves<NG>(t1, vc + v_next);
+            lds_halves<NG>(t8, vc + 8 * (D / 2));
+            lds_halves<NG>(t9, vc + 8 * (D / 2) + v_next);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              const uint32_t lo = __byte_perm(t0[g / 2], t1[g / 2], g % 2 ? 0x7632 : 0x5410);
+              const uint32_t hi = __byte_perm(t8[g / 2], t9[g / 2], g % 2 ? 0x7632 : 0x5410);
+              const uint32_t a0[4] = {codes_fp16<kCentred, 0>(lo), codes_fp16<kCentred, 1>(lo), codes_fp16<kCentred, 0>(hi), codes_fp16<kCentred, 1>(hi)};
+              const uint32_t a1[4] = {codes_fp16<kCentred, 2>(lo), codes_fp16<kCentred, 3>(lo), codes_fp16<kCentred, 2>(hi), codes_fp16<kCentred, 3>(hi)};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t b0 = kHalf ? pb[nt][g][0] & keep : pb[nt][g][0], b1 = kHalf ? pb[nt][g][1] & keep : pb[nt][g][1];
+                mma16816<__half>(o[nt][g][0], a0, b0, b1);
+                mma16816<__half>(o[nt][g][1], a1, b0, b1);
+              }
             }
           }
         }
@@ -867,7 +897,11 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         top[nt][x] = kNoKey;
-        for (int w = 0; w < 4; ++w) top[nt][x] = max_nan(top[nt][x], ml[(w * kRows + nt * 8 + 2 * c + x) * 2]);
+        for (int w = 0; w < 4; ++w) {
+          const float* at_row = ml + (w * kRows + nt * 8 + (kHalf ? (2 * c + x) & 3 : 2 * c + x)) * 2;
+          top[nt][x] = max_nan(top[nt][x], at_row[0]);
+          if (kHalf) top[nt][x] = max_nan(top[nt][x], at_row[8]);
+        }
       }
     for (int w = 0; w < 2; ++w) {  // in a fixed order: the same sum every time
       if (w == side) {
@@ -896,16 +930,27 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
       if (at.page == 0) by->x = blockIdx.x;
       if (at.page + run == at.pages) by->y = blockIdx.x;
     }
-    for (int i = threadIdx.x; i < kRows * D / 8; i += 128) {
+    for (int i = threadIdx.x; i < kUsedRows * D / 8; i += 128) {
       const int row = i / (D / 8), ch = i % (D / 8) * 8, rg = row0 + row;
       if (rg >= n_rows) continue;
       float mm = kNoKey, ll = 0.f;
-      for (int w = 0; w < 4; ++w) mm = max_nan(mm, ml[(w * kRows + row) * 2]);
-      for (int w = 0; w < 4; ++w) ll += ml[(w * kRows + row) * 2 + 1] * fast_exp2(ml[(w * kRows + row) * 2] - mm);
-      const float* even = join + row * D + ch;
-      const float* odd = even + kRows * D;
-      const float4 x = add4(*reinterpret_cast<const float4*>(even), *reinterpret_cast<const float4*>(odd));
-      const float4 y = add4(*reinterpret_cast<const float4*>(even + 4), *reinterpret_cast<const float4*>(odd + 4));
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+#pragma unroll
+      for (int set = 0; set < 3 - kJ; ++set)
+        for (int w = 0; w < 4; ++w) mm = max_nan(mm, ml[(w * kRows + set * 4 + row) * 2]);
+#pragma unroll
+      for (int set = 0; set < 3 - kJ; ++set) {
+        for (int w = 0; w < 4; ++w) {
+          const float* at_row = ml + (w * kRows + set * 4 + row) * 2;
+          ll += at_row[1] * fast_exp2(at_row[0] - mm);
+        }
+#pragma unroll
+        for (int pr = 0; pr < 2; ++pr) {
+          const float* from = join + (pr * kRows + set * 4 + row) * D + ch;
+          x = add4(x, *reinterpret_cast<const float4*>(from));
+          y = add4(y, *reinterpret_cast<const float4*>(from + 4));
+        }
+      }
       if (whole) {
         const int t = rg / G, h = head * G + rg % G;
         const float inv = ll == 0.f ? 0.f : 1.f / ll;
@@ -1009,38 +1054,6 @@ static int kv4_tiles(int T, int G, int D) { return T * G > 8 && D <= 128 ? 2 : 1
 static int kv4_blocks(int D, int nt) { return kSmCount * (D / kGroup * nt <= 4 ? 4 : D / kGroup * nt <= 6 ? 3 : 2); }
 static bool kv4_dim(int D) { return D == 64 || D == 96 || D == 128 || D == 192 || D == 256; }
 
-template <typename T, int NG, int NT>
-static int launch_kv4_attn(const Kv4AttnParams& p, cudaStream_t s) {
-  using Cfg = Kv4Cfg<NG, NT>;
-  auto kern = kv4_attn_kernel<T, NG, NT>;
-  static bool attr_done[kMaxDevices] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) { cudaGetLastError(); return RFA_ERR_CUDA; }
-  if (!attr_done[dev]) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes) != cudaSuccess) {
-      cudaGetLastError();
-      return RFA_ERR_CUDA;
-    }
-    attr_done[dev] = true;
-  }
-  const int rc = launch_chained(kern, static_cast<unsigned>(p.blocks), 128, Cfg::kSmemBytes, s, p);
-  if (rc != RFA_OK) return rc;
-  return launch_chained(kv4_join_kernel<T>, static_cast<unsigned>(p.B) * p.units * Cfg::kRows, 128, 0, s, p,
-                        static_cast<int>(Cfg::kRows));
-}
-
-template <typename T>
-static int dispatch_kv4_attn(const Kv4AttnParams& p, int nt, cudaStream_t s) {
-  switch (p.D) {
-    case 64: return nt == 2 ? launch_kv4_attn<T, 2, 2>(p, s) : launch_kv4_attn<T, 2, 1>(p, s);
-    case 96: return nt == 2 ? launch_kv4_attn<T, 3, 2>(p, s) : launch_kv4_attn<T, 3, 1>(p, s);
-    case 128: return nt == 2 ? launch_kv4_attn<T, 4, 2>(p, s) : launch_kv4_attn<T, 4, 1>(p, s);
-    case 192: return launch_kv4_attn<T, 6, 1>(p, s);
-    case 256: return launch_kv4_attn<T, 8, 1>(p, s);
-    default: return RFA_ERR_UNSUPPORTED;
-  }
-}
-
 // f(a value of the 16-bit type, the number of channel groups)
 template <typename F>
 static int kv4_by_groups(int D, F&& f) {
@@ -1057,6 +1070,38 @@ template <typename F>
 static int kv4_by_type(int dtype, int D, F&& f) {
   if (dtype == RFA_DTYPE_BF16) return kv4_by_groups(D, [&](auto groups) { return f(__nv_bfloat16{}, groups); });
   return kv4_by_groups(D, [&](auto groups) { return f(__half{}, groups); });
+}
+
+template <typename T, int NG, int NT, bool kHalf = false>
+static int launch_kv4_attn(const Kv4AttnParams& p, cudaStream_t s) {
+  using Cfg = Kv4Cfg<NG, NT>;
+  auto kern = kv4_attn_kernel<T, NG, NT, kHalf>;
+  static bool attr_done[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) { cudaGetLastError(); return RFA_ERR_CUDA; }
+  if (!attr_done[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes) != cudaSuccess) {
+      cudaGetLastError();
+      return RFA_ERR_CUDA;
+    }
+    attr_done[dev] = true;
+  }
+  const int rc = launch_chained(kern, static_cast<unsigned>(p.blocks), 128, Cfg::kSmemBytes, s, p);
+  if (rc != RFA_OK) return rc;
+  return launch_chained(kv4_join_kernel<T>, static_cast<unsigned>(p.B) * p.units * Cfg::kRows, 128, 0, s, p,
+                        static_cast<int>(Cfg::kRows));
+}
+
+// Four query rows or fewer fold the columns (see the kernel); more take one or two column tiles.
+template <typename T>
+static int dispatch_kv4_attn(const Kv4AttnParams& p, int nt, cudaStream_t s) {
+  return kv4_by_groups(p.D, [&](auto groups) {
+    constexpr int NG = decltype(groups)::value;
+    if (p.T * (p.Hq / p.Hkv) <= 4) return launch_kv4_attn<T, NG, 1, true>(p, s);
+    if constexpr (NG <= 4)
+      if (nt == 2) return launch_kv4_attn<T, NG, 2>(p, s);
+    return launch_kv4_attn<T, NG, 1>(p, s);
+  });
 }
 
 static int kv4_check(const void* codes, const void* meta, int n_pages, const int* table, int max_pages, const int* rows, int B,
