@@ -124,8 +124,7 @@ __global__ void __launch_bounds__(256) bwd_prepare_kernel(const T* __restrict__ 
     const int s = static_cast<int>(bs % Spad);
     const int b = static_cast<int>(bs / Spad);
     const size_t stat = (static_cast<size_t>(b) * Hq + h) * Spad + s;
-    // a row that saw no key (lse -inf: padding of a document mask, whose dout may be anything) has delta 0 and weights 0
-    const bool real = in_range && s < Sq && lse[stat] != -INFINITY;
+    const bool real = in_range && s < Sq;
     float acc = 0.f;
     if (real && gl < vec_per_row) {
       const size_t row_off = ((static_cast<size_t>(b) * Sq + s) * Hq + h) * D;
@@ -135,8 +134,11 @@ __global__ void __launch_bounds__(256) bwd_prepare_kernel(const T* __restrict__ 
     }
     for (int o = gsz >> 1; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
     if (in_range && gl == 0) {
-      delta[stat] = real ? acc : 0.f;
-      lse2[stat] = real ? lse[stat] * 1.4426950408889634f : INFINITY;
+      // a row that saw no key (lse -inf: padding of a document mask, whose dout may be anything) has delta 0 and weights 0
+      const float l = real ? lse[stat] : -INFINITY;
+      const bool sees = l != -INFINITY;
+      delta[stat] = sees ? acc : 0.f;
+      lse2[stat] = sees ? l * 1.4426950408889634f : INFINITY;
     }
   }
 }
