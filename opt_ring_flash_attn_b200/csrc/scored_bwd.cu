@@ -579,14 +579,16 @@ __global__ void __launch_bounds__(640, 1)
                 if (kLinear) bias = add2(bias, step);
                 else y2 = add2(y2, pack_f2(slope * fabsf(static_cast<float>(d + 2 * k)), slope * fabsf(static_cast<float>(d + 2 * k + 1))));
               }
-              float jac0 = 1.f, jac1 = 1.f;
+              uint64_t jac2 = 0;
               if constexpr (kKind == 2) {
-                // cap tanh(x / cap) = cap - 2 cap h and 1 - tanh^2 = 4 h (1 - h) with h = 1 / (exp(2 x / cap) + 1)
-                const float h0 = fast_rcp(fast_exp2(__uint_as_float(r[c][2 * k]) * in_scale) + 1.f);
-                const float h1 = fast_rcp(fast_exp2(__uint_as_float(r[c][2 * k + 1]) * in_scale) + 1.f);
-                y2 = fma2(pack_f2(h0, h1), pack_f2(2.f * cap_log2, 2.f * cap_log2), y2);
-                jac0 = 4.f * fmaf(-h0, h0, h0);
-                jac1 = 4.f * fmaf(-h1, h1, h1);
+                // cap tanh(x / cap) = cap - cap g and 1 - tanh^2 = g (2 - g) with g = 2 / (exp(2 x / cap) + 1)
+                float a0, a1;
+                unpack_f2(mul2(pack_u2(r[c][2 * k], r[c][2 * k + 1]), pack_f2(in_scale, in_scale)), a0, a1);
+                const uint64_t half2 = pack_f2(0.5f, 0.5f);
+                unpack_f2(fma2(pack_f2(fast_exp2(a0), fast_exp2(a1)), half2, half2), a0, a1);
+                const uint64_t g2 = pack_f2(fast_rcp(a0), fast_rcp(a1));
+                y2 = fma2(g2, pack_f2(cap_log2, cap_log2), y2);
+                jac2 = mul2(g2, sub2(pack_f2(2.f, 2.f), g2));
               } else {
                 y2 = fma2(pack_u2(r[c][2 * k], r[c][2 * k + 1]), nscale2, y2);
               }
@@ -599,7 +601,13 @@ __global__ void __launch_bounds__(640, 1)
                 if (static_cast<unsigned>(qp + 1) >= static_cast<unsigned>(width)) e1 = 0.f;
               }
               u[k] = Pack2<T>::pack(e0, e1);
-              pk[c * 16 + k] = kKind == 2 ? Pack2<T>::pack(e0 * jac0, e1 * jac1) : u[k];
+              if constexpr (kKind == 2) {
+                float w0, w1;
+                unpack_f2(mul2(pack_f2(e0, e1), jac2), w0, w1);
+                pk[c * 16 + k] = Pack2<T>::pack(w0, w1);
+              } else {
+                pk[c * 16 + k] = u[k];
+              }
             }
             // P^T (16 bit, two per column) goes over the start of this group's own S^T columns, all of which are in registers
             tmem_st16(a_s + c * 16, u);
