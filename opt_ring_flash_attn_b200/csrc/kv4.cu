@@ -20,7 +20,10 @@ constexpr int kSmCount = 148;
 constexpr int kMaxParts = kSmCount * 4;  // blocks of a launch at most
 
 // ----------------------------------------------------------------------------
-// Append and read-back: four lanes per group, eight channels each.  Bound by memory: 2 x 16 bytes in and 2 x 5 out per lane.
+// Append and read-back: four lanes per group, eight channels each.  8192 tokens of 8 heads of 128 in 22 and 13 us, 2.0 and 3.3 TB/s
+// of 44 MB each: bound by instructions (issue 72 % busy, the logic unit 52 and 64 %), of which a border between two codes in one
+// group of many takes a fourth.  One token of 64 sequences: 6.3 us for both, launches.  Four tokens per lane instead of one, to
+// share the index arithmetic, keep too few warps resident: 33 us.
 // ----------------------------------------------------------------------------
 template <typename T>
 struct Kv4Type;
@@ -238,6 +241,13 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(T* __restrict__ k, T* _
 // how few of its operations a code needs, and the pages of all sequences and heads are dealt out evenly: with units (b, kv
 // head, tile of query rows) laid end to end, block i takes pages [i q, (i + 1) q) of them all, whatever the lengths are.  A
 // unit that several blocks share is joined by a second kernel from at most two partial results per block.
+//
+// Measured (pages scattered, lengths to 8192 / two of 131072; 32/8 heads of 128): 92 and 79 us for 335 and 286 MB, 3.7 TB/s; the
+// longer the cache the nearer to 4.7 TB/s (8 x as long), the copies alone take 72 and 62.  The logic unit is 52 % busy, issue
+// 55 %; some 15 us are the start, the joining of warps and the second launch.  One sequence of 1000: 12 us.  Steps on the way:
+// a fifth warp for the copies 144 / 118 us (it costs registers: five warps on four schedulers); products in e4m3 161 / 126; fp16
+// subnormals 141 / 104; parts of a unit read with loads in flight instead of in turn 104 -> 89; a cost per unit in the sharing
+// out 139 -> 97; columns folded 97 / 84 -> 92 / 79.  More work for the warps that an SM favours (the older ones) changes nothing.
 //
 // A block has two pairs of warps; a pair takes every other page of a run, a warp 32 of its 64 tokens, and the pair's first
 // warp keeps its pages coming through a ring of its own.  Tokens are the 16 rows, query rows (tokens x heads of the group, 8
