@@ -264,8 +264,8 @@ int rfa_document_mask(const int* cu, const int* prefix, int cu_rows, int n_docs,
  * rfa_fwd_hop, rfa_bwd_hop and rfa_bwd_local with modified scores, for blocks of equal length S (q, k, v of [B,S,H,D]).
  * State, scratch and results as there; rfa_bwd_prepare and rfa_bwd_dq_finalize serve both.  `args` is host memory, read
  * before the call returns.  Padding rows of q, k, v and dout may hold anything; their out and gradients are zero.
- *  dq_order  NULL, or rfa_dq_order_elems(B,S,Hq,D) counters: bit-reproducible gradients (every tile that the causal rule
- *            alone would visit is visited then, whatever the mask leaves of it)
+ *  dq_order  NULL, or rfa_dq_order_elems(B,S,Hq,D) counters: bit-reproducible gradients (with a mask every tile is visited
+ *            then, whatever the mask leaves of it)
  */
 int rfa_scored_fwd_hop(const void* q, const void* k, const void* v, float* acc, float* m, float* l, void* out, float* lse,
                        int B, int S, int Hq, int Hkv, int D, int dtype, const rfa_score_args* args, int first, int last,

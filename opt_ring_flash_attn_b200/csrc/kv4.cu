@@ -273,7 +273,8 @@ struct Kv4AttnParams {
   float* lse;
   float* part_o;   // [2 * blocks][rows][D]
   float* part_ml;  // [2 * blocks][rows][2]
-  int2* shared_by; // [B][units]: first and last block of the unit
+  int* opened;     // [blocks]: the unit that the block begins and leaves to others, or -1
+  int* last_block; // [B][units]: the block that ends the unit
   long long q_b, q_t, q_h;  // strides of q, in elements
   int B, T, Hq, Hkv, D;
   int n_pages, max_pages, units, blocks;  // units: (kv head, row tile) pairs of a sequence
@@ -516,7 +517,7 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
   Kv4Cursor at = kv4_seek(p, [&](int all) { return block_start(p, all, blockIdx.x); }, total, skip);
   int work = block_start(p, total, blockIdx.x + 1) - block_start(p, total, blockIdx.x);
   __syncthreads();  // the barriers are ready
-  if (skip_flag != 0 || work <= 0) return;
+  if (skip_flag != 0) return;
   const int n_row_tiles = p.units / p.Hkv;
   uint8_t* const ring = smem + pair * (kRing * Cfg::kStageBytes);
 
@@ -547,7 +548,7 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
     next_page = f.settle(p, pair);
     return true;
   };
-  if (side == 0 && lane == 0) {
+  if (side == 0 && lane == 0 && work > 0) {
     Kv4Fetch& f = fetcher[pair];
     int f_skip = skip;
     f.at = at;
@@ -566,7 +567,8 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
   const uint32_t first_set = r < 4 ? 0xffffffffu : 0;  // kHalf: columns (rows of the B operand's lanes) of the first set
   const int G = p.Hq / p.Hkv;
   const int n_rows = p.T * G;
-  int n = 0;  // pages of the pair so far
+  int n = 0;         // pages of the pair so far
+  int opened = -1;
   while (work > 0) {
     const int run = at.take(work, skip);
     if (run == 0) {  // the share ends before the first page of this unit, or begins behind the last of the one before
@@ -935,11 +937,9 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
     }
     const bool whole = at.page == 0 && run == at.pages;
     const int slot = 2 * blockIdx.x + (at.page > 0 ? 0 : 1);
-    if (threadIdx.x == 0) {
-      int2* by = p.shared_by + static_cast<size_t>(at.b) * p.units + at.u;
-      if (at.page == 0) by->x = blockIdx.x;
-      if (at.page + run == at.pages) by->y = blockIdx.x;
-    }
+    if (at.page == 0 && !whole) opened = at.b * p.units + at.u;
+    if (threadIdx.x == 0 && at.page > 0 && at.page + run == at.pages)
+      p.last_block[static_cast<size_t>(at.b) * p.units + at.u] = blockIdx.x;
     for (int i = threadIdx.x; i < kUsedRows * D / 8; i += 128) {
       const int row = i / (D / 8), ch = i % (D / 8) * 8, rg = row0 + row;
       if (rg >= n_rows) continue;
@@ -979,6 +979,15 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
     __syncthreads();  // the next run writes the same buffers
     at.next_unit(p);
   }
+  if (threadIdx.x == 0) p.opened[blockIdx.x] = opened;
+  // sequences without keys
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+    if (kv4_len(p, b) > 0) continue;
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + static_cast<size_t>(b) * p.T * p.Hq * D);
+    for (int i = threadIdx.x; i < p.T * p.Hq * (D / 8); i += 128) dst[i] = make_uint4(0, 0, 0, 0);
+    if (p.lse)
+      for (int i = threadIdx.x; i < p.T * p.Hq; i += 128) p.lse[static_cast<size_t>(b) * p.Hq * p.T + i] = -INFINITY;
+  }
   if (threadIdx.x == 0 && abort_flag) {
     // Give copies that are still in flight time to land before the block's shared memory is released.
     const unsigned long long t0 = global_timer_ns();
@@ -987,29 +996,23 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
   }
 }
 
-// One block per (b, unit, row): joins the partial results of a unit that several blocks shared, and answers for sequences
-// without keys.
+// Joins the partial results of the units that several blocks shared: one block per query row and block of the other kernel,
+// which has something to do where that one began a unit and left it.
 template <typename T>
-__global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttnParams p, int tile_rows) {
-  // what does not depend on the other kernel comes before the wait for it (it has waited for the lengths itself)
+__global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttnParams p, int tile_rows, int used_rows) {
+  pdl_wait();
+  const int row = blockIdx.x % used_rows, c0 = blockIdx.x / used_rows;
+  const int unit = p.opened[c0];
+  if (unit < 0 || unit >= p.B * p.units) return;
+  const int c1 = p.last_block[unit];
+  if (c1 <= c0 || c1 >= p.blocks) return;  // the other kernel gave up
   const int n_row_tiles = p.units / p.Hkv, G = p.Hq / p.Hkv;
-  const int row = blockIdx.x % tile_rows;
-  const int u = blockIdx.x / tile_rows % p.units, b = blockIdx.x / tile_rows / p.units;
+  const int u = unit % p.units, b = unit / p.units;
   const int rg = u % n_row_tiles * tile_rows + row;
   if (rg >= p.T * G) return;
   const int t = rg / G, h = u / n_row_tiles * G + rg % G;
   T* dst = static_cast<T*>(p.out) + ((static_cast<size_t>(b) * p.T + t) * p.Hq + h) * p.D;
   float* lse = p.lse ? p.lse + (static_cast<size_t>(b) * p.Hq + h) * p.T + t : nullptr;
-  const int pages = pages_of(kv4_len(p, b));
-  pdl_wait();
-  if (pages == 0) {
-    if (threadIdx.x < p.D / 2) reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = 0;
-    if (lse && threadIdx.x == 0) *lse = -INFINITY;
-    return;
-  }
-  const int2 by = p.shared_by[static_cast<size_t>(b) * p.units + u];
-  const int c0 = by.x, c1 = by.y;
-  if (c0 >= c1 || c0 < 0 || c1 >= p.blocks) return;  // written by the block itself (or the other kernel gave up)
   // Maximum and weights of the parts first, by all threads; then each warp sums every fourth part, loads of
   // several parts in flight (one thread per channel pair walking all parts took 29 us for 37 of them).
   __shared__ float weight[kMaxParts];
@@ -1098,8 +1101,10 @@ static int launch_kv4_attn(const Kv4AttnParams& p, cudaStream_t s) {
   }
   const int rc = launch_chained(kern, static_cast<unsigned>(p.blocks), 128, Cfg::kSmemBytes, s, p);
   if (rc != RFA_OK) return rc;
-  return launch_chained(kv4_join_kernel<T>, static_cast<unsigned>(p.B) * p.units * Cfg::kRows, 128, 0, s, p,
-                        static_cast<int>(Cfg::kRows));
+  const int rows = p.T * (p.Hq / p.Hkv);
+  const int used = rows < Cfg::kRows ? rows : Cfg::kRows;
+  return launch_chained(kv4_join_kernel<T>, static_cast<unsigned>(p.blocks) * used, 128, 0, s, p, static_cast<int>(Cfg::kRows),
+                        used);
 }
 
 // Four query rows or fewer fold the columns (see the kernel); more take one or two column tiles.
@@ -1183,7 +1188,7 @@ extern "C" size_t rfa_kv4_scratch_elems(int B, int T, int Hq, int Hkv, int D) {
   if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || !kv4_dim(D)) return 0;
   const int nt = kv4_tiles(T, Hq / Hkv, D);
   const size_t units = (static_cast<size_t>(T) * (Hq / Hkv) + 8 * nt - 1) / (8 * nt) * Hkv;
-  return static_cast<size_t>(2) * kv4_blocks(D, nt) * 8 * nt * (D + 2) + 2 * units * B;
+  return static_cast<size_t>(2) * kv4_blocks(D, nt) * 8 * nt * (D + 2) + kv4_blocks(D, nt) + units * B;
 }
 
 extern "C" int rfa_kv4_attn(const void* q, const long long* q_strides, const void* codes, const void* meta, int n_pages,
@@ -1232,7 +1237,8 @@ extern "C" int rfa_kv4_attn(const void* q, const long long* q_strides, const voi
   p.blocks = static_cast<int>(most < kv4_blocks(D, nt) ? most : kv4_blocks(D, nt));
   p.part_o = scratch;
   p.part_ml = scratch + static_cast<size_t>(2) * p.blocks * rows * D;
-  p.shared_by = reinterpret_cast<int2*>(p.part_ml + static_cast<size_t>(2) * p.blocks * rows * 2);
+  p.opened = reinterpret_cast<int*>(p.part_ml + static_cast<size_t>(2) * p.blocks * rows * 2);
+  p.last_block = p.opened + p.blocks;
   p.scale_log2 = softmax_scale * kLog2e;
   p.cap_log2 = softcap * kLog2e;
   p.cap_in = softcap > 0.f ? 2.f * softmax_scale * kLog2e / softcap : 0.f;

@@ -90,6 +90,6 @@ def test_abi_refuses_bad_arguments():
     assert att(T=1 << 30) == -5
     assert lib.rfa_kv4_scratch_elems(1, 1, 4, 3, 64) == 0 and lib.rfa_kv4_scratch_elems(1, 1, 4, 2, 80) == 0
     assert lib.rfa_kv4_scratch_elems(0, 1, 4, 2, 64) == 0
-    # two parts of 8 rows per block at least, and two numbers per unit
-    assert lib.rfa_kv4_scratch_elems(5, 1, 4, 2, 128) - lib.rfa_kv4_scratch_elems(4, 1, 4, 2, 128) == 2 * 2
+    # two parts of 8 rows per block at least, and a number per unit
+    assert lib.rfa_kv4_scratch_elems(5, 1, 4, 2, 128) - lib.rfa_kv4_scratch_elems(4, 1, 4, 2, 128) == 2
     assert lib.rfa_kv4_scratch_elems(1, 1, 4, 2, 128) >= 2 * 148 * 8 * 130
