@@ -270,6 +270,14 @@ int rfa_document_mask(const int* cu, const int* prefix, int cu_rows, int n_docs,
 int rfa_scored_fwd_hop(const void* q, const void* k, const void* v, float* acc, float* m, float* l, void* out, float* lse,
                        int B, int S, int Hq, int Hkv, int D, int dtype, const rfa_score_args* args, int first, int last,
                        int* status, void* stream);
+/* The forward pass of a sequence that has no ring: one launch, or, where few heads leave SMs idle, two with the keys of a row
+ * shared by several CTAs.  scratch: rfa_scored_fwd_scratch_elems floats on a 16-byte boundary, or NULL (one launch always; also
+ * where that is 0).  typical_keys: how many keys a row is expected to see at most (0: all of them); it only guides the choice,
+ * and both calls have to get the same. */
+size_t rfa_scored_fwd_scratch_elems(int B, int S, int Hq, int D, int causal, int typical_keys);
+int rfa_scored_fwd_local(const void* q, const void* k, const void* v, void* out, float* lse, float* scratch, int B, int S,
+                         int Hq, int Hkv, int D, int dtype, const rfa_score_args* args, int typical_keys, int* status,
+                         void* stream);
 int rfa_scored_bwd_hop(const void* q, const void* k, const void* v, const void* dout, const float* lse2,
                        const float* delta, float* dq_acc, float* dkdv_out, int B, int S, int Hq, int Hkv, int D, int dtype,
                        const rfa_score_args* args, int* dq_order, int* status, void* stream);

@@ -52,6 +52,8 @@ SIGNATURES = {
     "rfa_mask_elems": (_sz, [_i] * 3),
     "rfa_document_mask": (_i, [_vp] * 2 + [_i] * 6 + [_vp] * 2),
     "rfa_scored_fwd_hop": (_i, [_vp] * 8 + [_i] * 6 + [_vp] + [_i] * 2 + [_vp] * 2),
+    "rfa_scored_fwd_scratch_elems": (_sz, [_i] * 6),
+    "rfa_scored_fwd_local": (_i, [_vp] * 6 + [_i] * 6 + [_vp, _i] + [_vp] * 2),
     "rfa_scored_bwd_hop": (_i, [_vp] * 8 + [_i] * 6 + [_vp] * 4),
     "rfa_scored_bwd_local": (_i, [_vp] * 13 + [_i] * 6 + [_vp] * 4),
     "rfa_kv4_scratch_elems": (_sz, [_i] * 5),
@@ -271,6 +273,22 @@ def scored_fwd_hop(q, k, v, acc, m, l, out, lse, args: ScoreArgs, first: bool, l
                                        lse.data_ptr(), B, S, Hq, k.shape[2], D, DTYPE_CODES[q.dtype], ctypes.byref(args),
                                        int(first), int(last), status.data_ptr(), _stream(stream, q))
     _check(rc, "rfa_scored_fwd_hop")
+
+
+@functools.lru_cache(maxsize=256)
+def scored_fwd_scratch_elems(B: int, S: int, Hq: int, D: int, causal: bool, typical_keys: int) -> int:
+    """Floats of scratch that :func:`scored_fwd_local` wants; 0: none."""
+    return load().rfa_scored_fwd_scratch_elems(B, S, Hq, D, int(causal), typical_keys)
+
+
+def scored_fwd_local(q, k, v, out, lse, scratch, args: ScoreArgs, typical_keys: int, status, stream=None) -> None:
+    """The forward pass of a sequence without a ring (``rfa_scored_fwd_local``)."""
+    B, S, Hq, D = q.shape
+    with _on_device(q):
+        rc = load().rfa_scored_fwd_local(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                                         _ptr(scratch), B, S, Hq, k.shape[2], D, DTYPE_CODES[q.dtype], ctypes.byref(args),
+                                         typical_keys, status.data_ptr(), _stream(stream, q))
+    _check(rc, "rfa_scored_fwd_local", kernels=1 if scratch is None else 2)
 
 
 def scored_bwd_hop(q, k, v, dout, lse2, delta, dq_acc, dkdv_out, args: ScoreArgs, status, stream=None,

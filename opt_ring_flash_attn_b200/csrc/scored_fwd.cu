@@ -11,6 +11,7 @@
 //  * A tile inside every row's interval needs no test; in the others a row compares the key with its own interval.
 //  * A row that has seen no key keeps the finite maximum kNoKey, and ends with out = 0, lse = -inf.
 //  * The issuing warp clears the padding rows of a V tile that holds the border between real rows and padding.
+//  * Without a ring, few heads share the key tiles of a row among several CTAs; a second kernel joins their states.
 //
 // Bound, as the plain hop, by the chain of one query tile (scores, softmax, products), which two tiles per CTA overlap; by the
 // start and end of CTAs where documents are short (5 us of a CTA's 30 at 13 key tiles a pair); and with a cap by the arithmetic
@@ -31,6 +32,8 @@ struct ScoredFwdParams {
   int B, S, Hq, Hkv, D;
   int Spad, nT;
   int first, last;
+  int nsplit;  // CTAs that share the key tiles of a pair of query tiles; each leaves its state in a copy of its own
+  size_t acc_split, ml_split;  // elements between the copies
   int* status;
   ScoreParams sc;
 };
@@ -158,15 +161,16 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
 
   // ---- tile coordinates: most work first, heads fastest ----
   const int nQs = (p.nT + NQ - 1) / NQ;
+  const int split = blockIdx.x % p.nsplit, block = blockIdx.x / p.nsplit;
   int b, h, qs;
   if (p.sc.has_mask) {
-    const int item = __ldg((NQ == 2 ? p.sc.mask.order_q2 : p.sc.mask.order_q) + blockIdx.x / p.Hq);
-    h = blockIdx.x % p.Hq;
+    const int item = __ldg((NQ == 2 ? p.sc.mask.order_q2 : p.sc.mask.order_q) + block / p.Hq);
+    h = block % p.Hq;
     b = item / nQs;
     qs = item % nQs;
   } else {
-    const int per_qs = p.Hq * p.B, rem = static_cast<int>(blockIdx.x) % per_qs;
-    qs = nQs - 1 - static_cast<int>(blockIdx.x) / per_qs;
+    const int per_qs = p.Hq * p.B, rem = block % per_qs;
+    qs = nQs - 1 - block / per_qs;
     b = rem / p.Hq;
     h = rem % p.Hq;
   }
@@ -193,6 +197,17 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
     }
   }
   if (j0 > j1) j0 = j1;  // nothing to do
+  if (p.nsplit > 1) {  // this CTA's run of them
+    const int n = j1 - j0, from = j0 + n * split / p.nsplit, to = j0 + n * (split + 1) / p.nsplit;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      t_lo[q] = max(t_lo[q], from);
+      t_hi[q] = min(t_hi[q], to);
+      if (t_lo[q] >= t_hi[q]) t_lo[q] = t_hi[q] = 0;
+    }
+    j0 = from;
+    j1 = to;
+  }
   const int nmax = j1 - j0;
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
@@ -397,8 +412,8 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
     const int row_g = m0_q + row;
     const uint32_t o_addr = tmem_base + lane_addr + Cfg::kTmO + q * DP;
     const size_t bh = static_cast<size_t>(b) * p.Hq + h;
-    float* acc_tile = p.acc + ((bh * p.nT + (qs * NQ + q)) * (DP / 4)) * 512;  // [DP/4][128][4]
-    const size_t ml_idx = bh * p.Spad + row_g;
+    float* acc_tile = p.acc + split * p.acc_split + ((bh * p.nT + (qs * NQ + q)) * (DP / 4)) * 512;  // [DP/4][128][4]
+    const size_t ml_idx = bh * p.Spad + row_g + split * p.ml_split;
 
     if (m0_q < p.S && !(n == 0 && !p.first && !p.last)) {
       bool ok = true;
@@ -695,6 +710,84 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
   }
 }
 
+constexpr int kMaxSplit = 16;
+
+// The states that the CTAs of a split left, into out and lse.  One block per tile of 128 rows: thread = row, and half of the
+// head dim.  A few megabytes; bound by latency.
+template <typename T>
+__global__ void __launch_bounds__(256) join_splits_kernel(const ScoredFwdParams p) {
+  pdl_wait();
+  const int tile = blockIdx.x % p.nT, h = blockIdx.x / p.nT % p.Hq, b = blockIdx.x / p.nT / p.Hq;
+  const int row = threadIdx.x & 127, row_g = tile * 128 + row;
+  if (row_g >= p.S) return;
+  const size_t bh = static_cast<size_t>(b) * p.Hq + h, ml_idx = bh * p.Spad + row_g;
+  float weight[kMaxSplit], top = kNoKey, sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMaxSplit; ++i)
+    if (i < p.nsplit) top = max_nan(top, p.m[ml_idx + i * p.ml_split]);
+#pragma unroll
+  for (int i = 0; i < kMaxSplit; ++i)
+    if (i < p.nsplit) {
+      const float m = p.m[ml_idx + i * p.ml_split];
+      weight[i] = m == kNoKey ? 0.f : fast_exp2(m - top);  // what stands beside that maximum is no sum
+      if (weight[i] != 0.f) sum = fmaf(weight[i], p.l[ml_idx + i * p.ml_split], sum);
+    }
+  const bool empty = top == kNoKey;
+  const float inv = 1.0f / sum;
+  const int DP = static_cast<int>(p.acc_split / p.ml_split), half = (p.D / 8 + 1) / 2 * 8;
+  const float* acc = p.acc + (bh * p.nT + tile) * (static_cast<size_t>(DP) * 128) + row * 4;
+  T* orow = static_cast<T*>(p.out) + ((static_cast<size_t>(b) * p.S + row_g) * p.Hq + h) * p.D;
+  const int begin = threadIdx.x < 128 ? 0 : half, end = threadIdx.x < 128 ? half : p.D;
+  for (int d = begin; d < end; d += 8) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+#pragma unroll
+    for (int i = 0; i < kMaxSplit; ++i)
+      if (i < p.nsplit && weight[i] != 0.f) {
+        const float* from = acc + i * p.acc_split + d / 4 * 512;
+        const float4 u = *reinterpret_cast<const float4*>(from), w = *reinterpret_cast<const float4*>(from + 512);
+        const float f = weight[i];
+        x = make_float4(fmaf(u.x, f, x.x), fmaf(u.y, f, x.y), fmaf(u.z, f, x.z), fmaf(u.w, f, x.w));
+        y = make_float4(fmaf(w.x, f, y.x), fmaf(w.y, f, y.y), fmaf(w.z, f, y.z), fmaf(w.w, f, y.w));
+      }
+    uint4 r = make_uint4(Pack2<T>::pack(x.x * inv, x.y * inv), Pack2<T>::pack(x.z * inv, x.w * inv),
+                         Pack2<T>::pack(y.x * inv, y.y * inv), Pack2<T>::pack(y.z * inv, y.w * inv));
+    if (empty) r = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(orow + d) = r;
+  }
+  if (threadIdx.x < 128) p.lse[ml_idx] = empty ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+}
+
+// Few heads: the longest row of tiles is as long as the pass, and most SMs wait.  Its key tiles are shared by so many CTAs that
+// it is no longer than the mean load of an SM, where that pays for the second launch and the states in between (some kJoin
+// tiles).  `typical_keys` (0: all) is how far a query may see: shorter rows need no split.  Measured, causal, us in one launch
+// and split (CTAs per row): S 2048, 1 head of 64 33 -> 23 (3); 8 heads of 128 35 -> 34, with a cap 62 -> 41 (3); S 4096, 4 heads
+// of 128 58 -> 39 (3); 8 heads 60 -> 52 (2); S 8192, 4 heads 109 -> 74 (2); S 16384, 1 head 204 -> 76 (4), 4 heads 217 (no
+// split).  At S 1536, 4 heads, the two are even (27).
+static int fwd_split(int B, int S, int Hq, int D, int causal, int typical_keys) {
+  constexpr int kSMs = 148;
+  constexpr double kCta = 3.0, kJoin = 5.0;  // in key tiles (1.6 us): start and end of a CTA; the join
+  const int pair = padded_head_dim(D) == 256 ? 1 : 2, nT = ceil_div(S, 128);
+  const double ctas = static_cast<double>(ceil_div(nT, pair)) * Hq * B;
+  double longest = nT;
+  if (typical_keys > 0 && typical_keys < S) longest = ceil_div(typical_keys, 128) + 1;
+  const double mean = causal ? 0.5 * longest : longest;
+  int best = 1;
+  double best_t = 0;
+  for (int n = 1; n <= kMaxSplit && (n == 1 || longest >= 4 * n); ++n) {
+    const double load = ctas * (mean + n * kCta) / kSMs, chain = longest / n + kCta;
+    const double t = (load > chain ? load : chain) + (n > 1 ? kJoin : 0);
+    if (n == 1 || t < 0.9 * best_t) {
+      best = n;
+      best_t = t;
+    }
+  }
+  return best;
+}
+// fp32 elements of one state: O, maxima and sums.
+static size_t state_elems(int B, int S, int Hq, int D) {
+  return static_cast<size_t>(B) * Hq * round_up(S, 128) * (padded_head_dim(D) + 2);
+}
+
 template <int DP, int BN, int NQ, int NS, typename T, int kKind>
 static int launch_scored_fwd(const void* q, const void* k, const void* v, const ScoredFwdParams& prm, int dtype,
                              cudaStream_t stream) {
@@ -721,7 +814,7 @@ static int launch_scored_fwd(const void* q, const void* k, const void* v, const 
     }
     attr_done[dev] = true;
   }
-  const unsigned grid = static_cast<unsigned>((prm.nT + NQ - 1) / NQ) * prm.Hq * prm.B;
+  const unsigned grid = static_cast<unsigned>((prm.nT + NQ - 1) / NQ) * prm.Hq * prm.B * prm.nsplit;
   return launch_chained(kern, grid, Cfg::kThreads, Cfg::kSmemBytes, stream, tq, tk, tv, prm);
 }
 
@@ -776,9 +869,64 @@ extern "C" int rfa_scored_fwd_hop(const void* q, const void* k, const void* v, f
   prm.nT = prm.Spad / 128;
   prm.first = first ? 1 : 0;
   prm.last = last ? 1 : 0;
+  prm.nsplit = 1;
+  prm.acc_split = prm.ml_split = 0;
   prm.status = status;
   if (static_cast<long long>(prm.nT) * Hq * B > INT_MAX) return RFA_ERR_TOO_LARGE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == RFA_DTYPE_BF16) return dispatch_scored_kind<__nv_bfloat16>(q, k, v, prm, dtype, s);
   return dispatch_scored_kind<__half>(q, k, v, prm, dtype, s);
+}
+
+extern "C" size_t rfa_scored_fwd_scratch_elems(int B, int S, int Hq, int D, int causal, int typical_keys) {
+  using namespace rfa;
+  if (B <= 0 || S <= 0 || Hq <= 0 || padded_head_dim(D) == 0) return 0;
+  const int n = fwd_split(B, S, Hq, D, causal, typical_keys);
+  return n > 1 ? n * state_elems(B, S, Hq, D) : 0;
+}
+
+extern "C" int rfa_scored_fwd_local(const void* q, const void* k, const void* v, void* out, float* lse, float* scratch, int B,
+                                    int S, int Hq, int Hkv, int D, int dtype, const rfa_score_args* args, int typical_keys,
+                                    int* status, void* stream) {
+  using namespace rfa;
+  if (!args) return RFA_ERR_INVALID_ARG;
+  if (scratch == nullptr || B <= 0 || S <= 0 || Hq <= 0 || padded_head_dim(D) == 0)
+    return rfa_scored_fwd_hop(q, k, v, nullptr, nullptr, nullptr, out, lse, B, S, Hq, Hkv, D, dtype, args, 1, 1, status, stream);
+  const int n = fwd_split(B, S, Hq, D, args->causal, typical_keys);
+  if (n == 1)
+    return rfa_scored_fwd_hop(q, k, v, nullptr, nullptr, nullptr, out, lse, B, S, Hq, Hkv, D, dtype, args, 1, 1, status, stream);
+  if (!q || !k || !v || !status || !out || !lse || Hkv <= 0 || Hq % Hkv != 0) return RFA_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(scratch) & 15u) || (reinterpret_cast<uintptr_t>(out) & 15u)) return RFA_ERR_INVALID_ARG;
+  if (dtype != RFA_DTYPE_BF16 && dtype != RFA_DTYPE_FP16) return RFA_ERR_UNSUPPORTED;
+  ScoredFwdParams prm;
+  int rc = make_score_params(args, B, S, &prm.sc);
+  if (rc != RFA_OK) return rc;
+  const size_t acc = static_cast<size_t>(B) * Hq * round_up(S, 128) * padded_head_dim(D);
+  const size_t ml = static_cast<size_t>(B) * Hq * round_up(S, 128);
+  prm.acc = scratch;
+  prm.m = scratch + n * acc;
+  prm.l = prm.m + n * ml;
+  prm.out = out;
+  prm.lse = lse;
+  prm.B = B;
+  prm.S = S;
+  prm.Hq = Hq;
+  prm.Hkv = Hkv;
+  prm.D = D;
+  prm.Spad = round_up(S, 128);
+  prm.nT = prm.Spad / 128;
+  prm.first = 1;
+  prm.last = 0;
+  prm.nsplit = n;
+  prm.acc_split = acc;
+  prm.ml_split = ml;
+  prm.status = status;
+  if (static_cast<long long>(prm.nT) * Hq * B * n > INT_MAX) return RFA_ERR_TOO_LARGE;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  rc = dtype == RFA_DTYPE_BF16 ? dispatch_scored_kind<__nv_bfloat16>(q, k, v, prm, dtype, s)
+                               : dispatch_scored_kind<__half>(q, k, v, prm, dtype, s);
+  if (rc != RFA_OK) return rc;
+  const unsigned grid = static_cast<unsigned>(prm.nT) * Hq * B;
+  return dtype == RFA_DTYPE_BF16 ? launch_chained(join_splits_kernel<__nv_bfloat16>, grid, 256, 0, s, prm)
+                                 : launch_chained(join_splits_kernel<__half>, grid, 256, 0, s, prm);
 }

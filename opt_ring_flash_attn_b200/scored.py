@@ -31,10 +31,11 @@ class DocumentMask:
     """Which keys the queries of a batch see (made by :func:`document_mask`).  It lives on the device; the forward and the
     backward passes of every layer that works on the same batch read it."""
 
-    def __init__(self, buffer, batch: int, seq_len: int, shards: int, causal: bool, has_prefix: bool):
+    def __init__(self, buffer, batch: int, seq_len: int, shards: int, causal: bool, has_prefix: bool, typical_keys: int = 0):
         self.buffer = buffer
         self.batch, self.seq_len, self.shards = batch, seq_len, shards
         self.causal, self.has_prefix = causal, has_prefix
+        self.typical_keys = typical_keys  # guides the split of long rows over CTAs (0: a row may see everything)
 
     @property
     def device(self) -> torch.device:
@@ -115,17 +116,20 @@ def document_mask(cu_seqlens: _Ints, seq_len: int, *, prefix_lens: Optional[_Int
         raise RuntimeError("document_mask runs on CUDA only (sm_100a kernels; there is no CPU path)")
     buffer = torch.empty(_native.mask_elems(batch, seq_len // shards, shards), dtype=torch.int32, device=device)
     _native.document_mask(cu, prefix, batch, seq_len // shards, shards, causal, buffer)
-    return DocumentMask(buffer, batch, seq_len, shards, bool(causal), prefix is not None)
+    # with n documents a long one holds some twice the mean; their borders stay on the device
+    return DocumentMask(buffer, batch, seq_len, shards, bool(causal), prefix is not None,
+                        min(seq_len, 2 * seq_len // (cu.shape[-1] - 1)))
 
 
 class _Scores:
     """What a pass does to its scores, and the kernel backend that the ring schedules call hop by hop."""
 
     def __init__(self, softmax_scale: float, softcap: float, slopes, causal: bool, mask_buffer, sees_later: bool,
-                 world: int, rank: int):
+                 world: int, rank: int, typical_keys: int = 0):
         self.scale, self.softcap, self.slopes, self.causal, self.mask = softmax_scale, softcap, slopes, causal, mask_buffer
         self.sees_later = sees_later  # some key behind a query may be visible: no hop can be left out
         self.world, self.rank, self._step = world, rank, 0
+        self.typical_keys = typical_keys  # what a long document holds, as far as the host knows (0: everything)
 
         self._args = _native.score_args(softmax_scale, softcap, slopes, causal, mask_buffer, world, rank, rank)
 
@@ -168,7 +172,9 @@ def _forward(group, q, k, v, sc: _Scores):
     B, S, Hq, _ = q.shape
     out = torch.empty_like(q)
     lse = torch.empty((B, Hq, _native.padded_seq(S)), dtype=torch.float32, device=q.device)
-    _native.scored_fwd_hop(q, k, v, None, None, None, out, lse, sc.args(0), True, True, ws.status)
+    n = _native.scored_fwd_scratch_elems(B, S, Hq, q.shape[3], sc.causal, sc.typical_keys)
+    scratch = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+    _native.scored_fwd_local(q, k, v, out, lse, scratch, sc.args(0), sc.typical_keys, ws.status)
     workspace.publish_status(ws, "scored_flash_attn forward")
     return out, lse
 
@@ -273,7 +279,8 @@ def _apply(q, k, v, softmax_scale, causal, softcap, alibi_slopes, mask, group) -
             raise ValueError(f"the mask is for a batch of {mask.batch} and {mask.seq_len} tokens on {mask.shards} ranks, "
                              f"the call has {B}, {S * world} and {world}")
     sees_later = not causal or (mask is not None and mask.has_prefix)
-    sc = _Scores(float(softmax_scale), softcap, slopes, causal, None if mask is None else mask.buffer, sees_later, world, rank)
+    buffer, typical = (None, 0) if mask is None else (mask.buffer, mask.typical_keys)
+    sc = _Scores(float(softmax_scale), softcap, slopes, causal, buffer, sees_later, world, rank, typical)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _ScoredFlashAttnFunc.apply(q, k, v, sc, group)
     return _call(_operand(q), _operand(k), _operand(v), sc, group)

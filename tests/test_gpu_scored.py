@@ -322,3 +322,56 @@ def test_malformed_borders_on_the_device_are_safe():
         mask = rfa.document_mask(torch.tensor(cu, device=DEV), S, prefix_lens=torch.tensor([1000] * (len(cu) - 1), device=DEV))
         got = _run(q, k, v, dout, causal=True, mask=mask)  # ends with a check of the status word
         assert got["out"].shape == q.shape
+
+
+SPLIT = [  # B, S, Hq, Hkv, D, dtype, causal, scores, borders, prefixes
+    (1, 2053, 2, 1, 64, BF, True, "both", None, None),
+    (1, 2500, 1, 1, 128, HF, False, "plain", None, None),
+    (2, 2300, 2, 2, 256, BF, True, "cap", None, None),
+    (1, 2048, 3, 1, 40, HF, False, "bias", None, None),
+    (1, 3000, 2, 2, 96, BF, True, "both", [7, 2900], [1200]),
+    # the second tile of a pair sees far more than the first; runs of key tiles that no row of a pair sees; padding only
+    (1, 3900, 2, 1, 64, HF, False, "plain", [0, 130, 3300], None),
+    (1, 3900, 1, 1, 128, BF, True, "cap", [300, 3500, 3600], [5, 90]),
+]
+
+
+@pytest.mark.parametrize("case", SPLIT, ids=lambda c: "-".join(map(str, c[1:5])) + "-" + c[7])
+def test_rows_shared_by_ctas(case):
+    """Few heads: the key tiles of a row are shared by several CTAs, whose states are joined."""
+    import opt_ring_flash_attn_b200 as rfa
+    from opt_ring_flash_attn_b200 import _native
+
+    B, S, Hq, Hkv, D, dt, causal, scores, cu, pre = case
+    sc = dict(SCORES[scores])
+    slopes = _slopes(Hq, signed=causal) if sc.pop("bias", False) else None
+    q, k, v, dout = inputs(16, B, S, Hq, Hkv, D, dt, DEV, std=1.5)
+    ref = reference(q, k, v, dout, visible(S, causal, cu, pre, DEV), slopes=slopes, **sc)
+    mask, typical = None, 0
+    if cu is not None:
+        mask = rfa.document_mask(cu, S, prefix_lens=pre, causal=causal, device=DEV)
+        typical = mask.typical_keys
+        real = torch.zeros(S, dtype=torch.bool, device=DEV)
+        real[cu[0]:cu[-1]] = True
+        for i, t in enumerate((q, k, v, dout)):
+            t[:, ~real] = [math.nan, math.inf, -math.inf, math.nan][i]
+    assert _native.scored_fwd_scratch_elems(B, S, Hq, D, causal, typical) > 0  # or the case tests nothing
+    got = _run(q, k, v, dout, causal=causal, mask=mask, alibi_slopes=slopes, **sc)
+    check(ref, **got)
+    again = _run(q, k, v, dout, causal=causal, mask=mask, alibi_slopes=slopes, **sc)
+    assert torch.equal(got["out"], again["out"]) and torch.equal(got["lse"], again["lse"])
+
+
+def test_no_number_reaches_its_row_from_any_share():
+    """A score that is no number makes its row NaN, whichever CTA meets it, and no other row."""
+    import opt_ring_flash_attn_b200 as rfa
+
+    S = 2100
+    q, k, v, _ = inputs(17, 1, S, 1, 1, 64, BF, DEV)
+    q[0, 2000, 0, 3] = math.nan
+    out, lse = rfa.scored_flash_attn_with_lse(q, k, v, causal=True)
+    rfa.check("test")
+    bad = torch.zeros(S, dtype=torch.bool, device=DEV)
+    bad[2000] = True
+    assert torch.equal(out.isnan().all(-1).flatten(), bad) and torch.equal(out.isnan().any(-1).flatten(), bad)
+    assert torch.equal(lse.isnan().flatten(), bad)

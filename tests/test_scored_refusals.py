@@ -100,3 +100,29 @@ def test_abi_refuses_bad_arguments():
     assert lib.rfa_mask_elems(0, 16, 1) == 0 and lib.rfa_mask_elems(1, 1 << 30, 4) == 0
     # intervals (4 x S, rounded to 4), hulls (8 per tile), orders (2 per tile, 1 per pair) and 2 borders per row
     assert lib.rfa_mask_elems(2, 300, 1) == 4 * 600 + 10 * 6 + 4 + 4
+
+
+def test_abi_of_the_shared_rows_refuses_bad_arguments():
+    import ctypes
+
+    lib = _native.load()
+    good = dict(softmax_scale=0.1, softcap=0.0, slopes=None, causal=True, mask=None)
+    args = lambda **kw: ctypes.byref(_native.score_args(**{**good, **kw}))  # noqa: E731
+    local = lambda a, q=256, S=4096, D=64, dt=0, scratch=256, H=1, Hkv=1: lib.rfa_scored_fwd_local(  # noqa: E731
+        q, 256, 256, 256, 256, scratch, 1, S, H, Hkv, D, dt, a, 0, 256, None)
+    assert lib.rfa_scored_fwd_scratch_elems(1, 4096, 1, 64, 1, 0) > 0  # or the calls below do not reach the split
+    assert local(None) == -1
+    assert local(args(softmax_scale=0.0)) == -1
+    assert local(args(), q=None) == -1
+    assert local(args(), scratch=264) == -1   # not on a 16-byte boundary
+    assert local(args(), Hkv=2) == -1
+    assert local(args(), S=0) == -1
+    assert local(args(), D=100) == -2
+    assert local(args(), dt=7) == -2
+    assert lib.rfa_scored_fwd_scratch_elems(1, 4096, 1, 100, 1, 0) == 0
+    assert lib.rfa_scored_fwd_scratch_elems(0, 4096, 1, 64, 1, 0) == 0
+    # one head of 64 over 4096 rows: copies of the state, each O, maxima and sums
+    assert lib.rfa_scored_fwd_scratch_elems(1, 4096, 1, 64, 1, 0) % (4096 * 66) == 0
+    # many heads, or documents that are short on average: one launch
+    assert lib.rfa_scored_fwd_scratch_elems(1, 4096, 32, 128, 1, 0) == 0
+    assert lib.rfa_scored_fwd_scratch_elems(1, 4096, 1, 64, 1, 200) == 0
