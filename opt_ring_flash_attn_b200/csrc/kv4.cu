@@ -1211,7 +1211,7 @@ extern "C" int rfa_kv4_attn(const void* q, const long long* q_strides, const voi
   const int nt = kv4_tiles(T, Hq / Hkv, D), rows = 8 * nt;
   const long long row_tiles = (static_cast<long long>(T) * (Hq / Hkv) + rows - 1) / rows;
   const long long units = row_tiles * Hkv;
-  if (static_cast<long long>(T) * Hq > INT_MAX / 2 || units * rows * B > INT_MAX / 2) return RFA_ERR_TOO_LARGE;
+  if (static_cast<long long>(T) * Hq * (D / 8) > INT_MAX - 128 || units * rows * B > INT_MAX / 2) return RFA_ERR_TOO_LARGE;
   Kv4AttnParams p{};
   p.q = q;
   p.codes = static_cast<const uint8_t*>(codes);

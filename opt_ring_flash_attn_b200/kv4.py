@@ -179,7 +179,7 @@ def kv4_attn(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, lens: 
       softmax_scale, softcap, alibi_slopes: as in :func:`scored_flash_attn`.
 
     Returns: out ``[B, T, H_q, D]``; rows that see no token are zero.  What the pages hold behind the last token does not
-    matter.  Results do not depend on how the work is split: the same call gives the same bits.
+    matter; the tokens themselves must be finite (of T > 1, a row may take up a NaN of a token behind it).  Results do not depend on how the work is split: the same call gives the same bits.
     """
     return _attn(q, cache, block_table, lens, softmax_scale, softcap, alibi_slopes, False)[0]
 

@@ -93,3 +93,11 @@ def test_abi_refuses_bad_arguments():
     # two parts of 8 rows per block at least, and a number per unit
     assert lib.rfa_kv4_scratch_elems(5, 1, 4, 2, 128) - lib.rfa_kv4_scratch_elems(4, 1, 4, 2, 128) == 2
     assert lib.rfa_kv4_scratch_elems(1, 1, 4, 2, 128) >= 2 * 148 * 8 * 130
+
+
+def test_abi_refuses_results_beyond_32_bit_indices():
+    """Query rows whose result has more than 2^31 vectors of 16 bytes per sequence."""
+    lib = _native.load()
+    st = (ctypes.c_longlong * 3)(64, 64, 64)
+    rc = lib.rfa_kv4_attn(256, st, 256, 256, 4, 256, 2, 256, 256, None, 256, 1, 1 << 26, 4, 2, 64, 0, 0.1, 0.0, None, 0, 256, None)
+    assert rc == -5
