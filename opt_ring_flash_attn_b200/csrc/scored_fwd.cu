@@ -16,7 +16,7 @@
 // Bound, as the plain hop, by the chain of one query tile (scores, softmax, products), which two tiles per CTA overlap; by the
 // start and end of CTAs where documents are short (5 us of a CTA's 30 at 13 key tiles a pair); and with a cap by the arithmetic
 // units, whose phases (cap, maximum, exponentials) one warpgroup goes through in turn.  Forward hop, causal, us: S 4096, 32/8
-// heads of 128: no change 140, bias 175, cap 233, both 258; 16 heads of 64: 64, 77, 119, 125; 16/8 heads of 256: 129, 153, 181, 212.
+// heads of 128: no change 140, bias 175, cap 233, both 258; 16 heads of 64: 64, 77, 117, 123; 16/8 heads of 256: 129, 153, 166, 189.
 // S 16384, 32/8 heads of 128, ten documents: 422 us = 832 TFLOP/s of visible pairs, tensor pipe 48 % busy.
 #include "fwd_common.cuh"
 #include "scored.cuh"
@@ -111,8 +111,15 @@ __device__ __forceinline__ float max32(const uint32_t (&r)[32]) {
   return max_nan(max3_nan(a, __uint_as_float(r[30]), __uint_as_float(r[31])), b);
 }
 
+// Softmax warpgroups per query tile.  Where a CTA holds one tile only (head dim 256) and there is a cap, two of them share its
+// keys, half each, and compare their maxima: one alone has a warp per scheduler for all of the arithmetic.  S 4096, 16/8 heads of
+// 256, us, one and two: cap 181, 166; with a bias too 210, 189.  Without a cap one keeps up with the copies and the products, and
+// the comparing costs: 129, 132; with a bias 153, 153.
+constexpr int fwd_share(int NQ, int kind) { return NQ == 1 && kind == 2 ? 2 : 1; }
+constexpr int fwd_threads(int NQ, int kind) { return 128 + NQ * fwd_share(NQ, kind) * 128; }
+
 template <int DP, int BN, int NQ, int NS, typename T, int kKind>
-__global__ void __launch_bounds__(128 + NQ * 128, 1)
+__global__ void __launch_bounds__(fwd_threads(NQ, kKind), 1)
     scored_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const ScoredFwdParams p) {
   using Cfg = FwdCfg<DP, BN, NQ, NS>;
@@ -120,6 +127,7 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
   constexpr bool kBf16 = Pack2<T>::kIsBf16;
   constexpr int kPvParts = (DP == 64) ? 2 : 4;     // P is handed to the issuer in parts, as in the plain hop
   constexpr int kPartChunks = BN / 32 / kPvParts;
+  constexpr int kShare = fwd_share(NQ, kKind);
   constexpr int kPolyEvery = (NQ == 2 && kKind < 2) ? kFwdPolyEvery : 0;  // a cap keeps the FMA pipe busy
 
   extern __shared__ uint8_t smem_raw[];
@@ -129,6 +137,8 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
   __shared__ uint64_t bar_s_full[NQ * NS];
   __shared__ uint64_t bar_p_ready[NQ * NS * kPvParts];
   __shared__ uint64_t bar_pv_done[NQ];
+  __shared__ uint64_t bar_pair[4];                          // two warps with the same rows of a tile
+  __shared__ float pair_value[kShare == 2 ? 2 : 1][128];    // maximum or sum of each half of a row's keys
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_flag, skip_flag;
 
@@ -151,6 +161,7 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
       for (int h = 0; h < kPvParts; ++h) mbar_init(&bar_p_ready[i * kPvParts + h], 128);
     }
     for (int i = 0; i < NQ; ++i) mbar_init(&bar_pv_done[i], 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&bar_pair[i], 2);
     mbar_fence_init();
   }
   if (warp == 0) {
@@ -397,7 +408,8 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
   } else {
     // =========================== softmax warpgroups ===========================
     if constexpr (NQ == 2) setmaxnreg_inc<Cfg::kSoftmaxRegs>();
-    const int q = (warp - 4) >> 2;
+    const int q = kShare == 2 ? 0 : (warp - 4) >> 2;
+    const int share = kShare == 2 ? (warp - 4) >> 2 : 0;  // half of the keys of a tile, and of the columns of O
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
@@ -409,6 +421,7 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
     const int full_lo_q = second ? full_lo[NQ - 1] : full_lo[0];
     const int full_hi_q = second ? full_hi[NQ - 1] : full_hi[0];
     const int n_c32 = (p.D + 31) / 32;
+    const int o_first = kShare == 2 && share == 1 ? (n_c32 + 1) / 2 : 0, o_end = kShare == 2 && share == 0 ? (n_c32 + 1) / 2 : n_c32;
     const int row_g = m0_q + row;
     const uint32_t o_addr = tmem_base + lane_addr + Cfg::kTmO + q * DP;
     const size_t bh = static_cast<size_t>(b) * p.Hq + h;
@@ -422,10 +435,10 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
       if (!p.first || n == 0) {  // the state of the hops before, or of none
         if (!p.first) {
           m_used = p.m[ml_idx];
-          l_sum = p.l[ml_idx];
+          if (share == 0) l_sum = p.l[ml_idx];
         }
 #pragma unroll 1
-        for (int c = 0; c < n_c32; ++c) {
+        for (int c = o_first; c < o_end; ++c) {
           uint32_t r[32];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
@@ -462,6 +475,17 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
       const float in_scale = kKind == 2 ? 2.f * scale_log2 / p.sc.cap : scale_log2;
       const TanhPoly tanh_poly(p.sc.scale / p.sc.cap, cap_log2);
       int direct = 0;  // tiles that take the formula at once
+      uint32_t pair_par = 0;
+      // Waits for the other warp with these rows; what either wrote before, tensor memory included, the other sees after.
+      auto pair_sync = [&]() {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_pair[quarter]);
+        const bool got = mbar_wait_warp(&bar_pair[quarter], pair_par, abort_p);
+        pair_par ^= 1;
+        tc_fence_after_sync();
+        return got;
+      };
 
 #pragma unroll 1
       for (int j = 0; j < n; ++j) {
@@ -469,11 +493,12 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
         const uint32_t par = (NS == 2) ? ((j >> 1) & 1) : (j & 1);
         if (!mbar_wait_warp(&bar_s_full[q * NS + sb], par, abort_p)) { ok = false; break; }
         tc_fence_after_sync();
-        const uint32_t s_addr = tmem_base + lane_addr + Cfg::kTmS + (q * NS + sb) * BN;
-        const int n0 = (j0 + t_first + j) * BN;
-        const bool masked = n0 < full_lo_q || n0 + BN > full_hi_q;
+        constexpr int NCH = BN / 32 / kShare, kKeys = BN / kShare;
+        const uint32_t s_tile = tmem_base + lane_addr + Cfg::kTmS + (q * NS + sb) * BN;
+        const uint32_t s_addr = s_tile + share * kKeys;
+        const int n0 = (j0 + t_first + j) * BN + share * kKeys;
+        const bool masked = n0 < full_lo_q || n0 + kKeys > full_hi_q;
 
-        constexpr int NCH = BN / 32;
         uint32_t r[NCH][32];
 #pragma unroll
         for (int c = 0; c < NCH; ++c) tmem_ld32(s_addr + c * 32, r[c]);
@@ -500,7 +525,7 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
         } else {
           // Keys all before or all after the queries: the distance is linear in the key, sign * (ahead - key).
           const int d0 = p.sc.q_pos + m0_q - p.sc.k_pos;  // of the first row
-          const bool before = n0 + BN - 1 <= d0, after = n0 >= d0 + 127;
+          const bool before = n0 + kKeys - 1 <= d0, after = n0 >= d0 + 127;
           const bool linear = before || after || slope == 0.f;
           const float sign_slope = before ? slope : after ? -slope : 0.f;
           const uint64_t step = pack_f2(2.f * sign_slope, 2.f * sign_slope);
@@ -543,7 +568,10 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
               cap32(r[c], tanh_poly, bias_of(c, 0.f), step, top[c]);
               mx = max_nan(mx, max32(r[c]));  // fills the gaps of the arithmetic; good where nothing changes any more
             }
-            const bool again = __any_sync(0xffffffffu, max3_nan(max_nan(top[0], top[1]), top[2], top[3]) > TanhPoly::kLimit);
+            float most = top[0];
+#pragma unroll
+            for (int c = 1; c < NCH; ++c) most = max_nan(most, top[c]);
+            const bool again = __any_sync(0xffffffffu, most > TanhPoly::kLimit);
             if (again) {
               int count = 0;
 #pragma unroll
@@ -554,10 +582,21 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
                   formula_chunk(c);
                   ++count;
                 }
-              direct = count >= 2 ? 8 : 0;  // a tile that left it in many places: the next ones will, too
+              direct = count >= NCH / 2 ? 8 : 0;  // a tile that left it in many places: the next ones will, too
             }
             if (again || masked || !linear) finish();
           }
+        }
+        if constexpr (kShare == 2) {
+          // The other half's maximum.  Its warp has read what this one left for the last tile once its first part of that P
+          // is there; and this half of P may only go over the other's scores once those are read.
+          if (j > 0 && !mbar_wait_warp(&bar_p_ready[((j - 1) & 1) * kPvParts + (1 - share) * (kPvParts / 2)], ((j - 1) >> 1) & 1, abort_p)) {
+            ok = false;
+            break;
+          }
+          pair_value[share][row] = mx;
+          if (!pair_sync()) { ok = false; break; }
+          mx = max_nan(mx, pair_value[1 - share][row]);
         }
         const float m_new = max_nan(m_used, kKind == 0 ? mx * scale_log2 : mx);
 
@@ -580,7 +619,7 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
             tc_fence_after_sync();
           }
 #pragma unroll 1
-          for (int c = 0; c < 2 * n_c32; ++c) {
+          for (int c = 2 * o_first; c < 2 * o_end; ++c) {
             uint32_t o16[16];
             tmem_ld16(o_addr + c * 16, o16);
             tmem_ld_wait16(o16);
@@ -589,6 +628,7 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
             tmem_st16(o_addr + c * 16, o16);
           }
           tmem_st_wait();
+          if (kShare == 2 && !pair_sync()) { ok = false; break; }  // all of O, before either's P is added to it
         }
 
         // P = exp2(z - m_used), packed to 16 bit over the start of S (rounded for the product, as in the plain hop; the sum
@@ -622,13 +662,13 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
             // the previous part of P has landed: the issuer may start O += P V on them
             tmem_st_wait();
             tc_fence_before_sync();
-            mbar_arrive(&bar_p_ready[(q * NS + sb) * kPvParts + c / kPartChunks - 1]);
+            mbar_arrive(&bar_p_ready[(q * NS + sb) * kPvParts + (share * NCH + c) / kPartChunks - 1]);
           }
-          tmem_st16(s_addr + c * 16, u);
+          tmem_st16(s_tile + (share * NCH + c) * 16, u);
         }
         tmem_st_wait();
         tc_fence_before_sync();
-        mbar_arrive(&bar_p_ready[(q * NS + sb) * kPvParts + kPvParts - 1]);
+        mbar_arrive(&bar_p_ready[(q * NS + sb) * kPvParts + (share + 1) * kPvParts / kShare - 1]);
         {
           float a0, a1, b0, b1;
           unpack_f2(lp2[0], a0, a1);
@@ -642,6 +682,11 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
       // the last product alone would also be satisfied by the phase before the one of tile n-2.
       if (NS == 2 && ok && n > 1) ok = mbar_wait_warp(&bar_pv_done[q], (n - 2) & 1, abort_p);
       if (ok && n > 0) ok = mbar_wait_warp(&bar_pv_done[q], (NS == 2) ? ((n - 1) & 1) : 0, abort_p);
+      if (kShare == 2 && ok) {  // every maximum has been read: the products of all P are done
+        pair_value[share][row] = l_sum;
+        ok = pair_sync();
+        l_sum = pair_value[0][row] + pair_value[kShare - 1][row];
+      }
       if (ok) {
         tc_fence_after_sync();
         l_sum += m_used - m_used;  // nothing, or NaN
@@ -651,7 +696,7 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
           const bool row_ok = row_g < p.S;
           T* orow = reinterpret_cast<T*>(p.out) + ((static_cast<size_t>(b) * p.S + row_g) * p.Hq + h) * p.D;
 #pragma unroll 1
-          for (int c = 0; c < n_c32; ++c) {
+          for (int c = o_first; c < o_end; ++c) {
             uint32_t r[32];
             tmem_ld32(o_addr + c * 32, r);
             tmem_ld_wait32(r);
@@ -670,10 +715,10 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
               }
             }
           }
-          if (row_ok) p.lse[ml_idx] = empty ? -INFINITY : (m_used + log2f(l_sum)) * 0.6931471805599453f;
+          if (row_ok && share == 0) p.lse[ml_idx] = empty ? -INFINITY : (m_used + log2f(l_sum)) * 0.6931471805599453f;
         } else {
 #pragma unroll 1
-          for (int c = 0; c < n_c32; ++c) {
+          for (int c = o_first; c < o_end; ++c) {
             uint32_t r[32];
             tmem_ld32(o_addr + c * 32, r);
             tmem_ld_wait32(r);
@@ -687,8 +732,10 @@ __global__ void __launch_bounds__(128 + NQ * 128, 1)
               *reinterpret_cast<float4*>(acc_tile + ((c * 8 + k) * 128 + row) * 4) = v;
             }
           }
-          p.m[ml_idx] = m_used;
-          p.l[ml_idx] = l_sum;
+          if (share == 0) {
+            p.m[ml_idx] = m_used;
+            p.l[ml_idx] = l_sum;
+          }
         }
       }
     }
@@ -810,12 +857,12 @@ static int launch_scored_fwd(const void* q, const void* k, const void* v, const 
       cudaFuncAttributes fa;
       e = cudaFuncGetAttributes(&fa, kern);
       if (e != cudaSuccess) { cudaGetLastError(); return RFA_ERR_CUDA; }
-      if (fa.numRegs * Cfg::kThreads < Cfg::kPoolRegs) return RFA_ERR_UNSUPPORTED;
+      if (fa.numRegs * fwd_threads(NQ, kKind) < Cfg::kPoolRegs) return RFA_ERR_UNSUPPORTED;
     }
     attr_done[dev] = true;
   }
   const unsigned grid = static_cast<unsigned>((prm.nT + NQ - 1) / NQ) * prm.Hq * prm.B * prm.nsplit;
-  return launch_chained(kern, grid, Cfg::kThreads, Cfg::kSmemBytes, stream, tq, tk, tv, prm);
+  return launch_chained(kern, grid, fwd_threads(NQ, kKind), Cfg::kSmemBytes, stream, tq, tk, tv, prm);
 }
 
 template <typename T, int kKind>
