@@ -16,7 +16,7 @@
 // Bound, as the plain hop, by the chain of one query tile (scores, softmax, products), which two tiles per CTA overlap; by the
 // start and end of CTAs where documents are short (5 us of a CTA's 30 at 13 key tiles a pair); and with a cap by the arithmetic
 // units, whose phases (cap, maximum, exponentials) one warpgroup goes through in turn.  Forward hop, causal, us: S 4096, 32/8
-// heads of 128: no change 140, bias 175, cap 233, both 258; 16 heads of 64: 64, 77, 117, 123; 16/8 heads of 256: 129, 153, 166, 189.
+// heads of 128: no change 140, bias 175, cap 219, both 245; 16 heads of 64: 64, 77, 113, 123; 16/8 heads of 256: 129, 153, 157, 187.
 // S 16384, 32/8 heads of 128, ten documents: 422 us = 832 TFLOP/s of visible pairs, tensor pipe 48 % busy.
 #include "fwd_common.cuh"
 #include "scored.cuh"
@@ -38,6 +38,10 @@ struct ScoredFwdParams {
   ScoreParams sc;
 };
 
+// What happens to the scores, as the kernels are instantiated: 0 nothing, 1 a bias, 2 a cap, 3 both.
+constexpr bool has_cap(int kind) { return kind >= 2; }
+constexpr bool has_bias(int kind) { return kind % 2 == 1; }
+
 // Scores of 32 keys in log2 units: the cap and the bias.  `bias` holds what is added to the first two keys, `step` what it
 // grows by from pair to pair (bias and step include the constant of the tanh).
 template <int kKind>
@@ -45,7 +49,7 @@ __device__ __forceinline__ void transform32(uint32_t (&r)[32], uint64_t scale2, 
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     uint64_t y;
-    if constexpr (kKind == 1) {
+    if constexpr (!has_cap(kKind)) {
       y = fma2(pack_u2(r[2 * i], r[2 * i + 1]), scale2, bias);
     } else {
       // cap * tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1); scale2 turns the raw score into the exponent, gain2 is
@@ -57,7 +61,7 @@ __device__ __forceinline__ void transform32(uint32_t (&r)[32], uint64_t scale2, 
       y = fma2(pack_f2(fast_rcp(e0), fast_rcp(e1)), gain2, bias);
     }
     unpack_u2(y, r[2 * i], r[2 * i + 1]);
-    bias = add2(bias, step);
+    if (has_bias(kKind)) bias = add2(bias, step);
   }
 }
 
@@ -65,22 +69,26 @@ __device__ __forceinline__ void transform32(uint32_t (&r)[32], uint64_t scale2, 
 // to even out the absolute error of the tanh: 3.5e-7).  The formula with exp2 and a reciprocal takes two turns on the
 // special-function unit per score, beside the one of the softmax, which makes it the unit that a tile waits for.  Forward hop,
 // scores of 3.2 on average, caps of 50 / 20 / 5 (where no, few and most chunks leave the range), by the formula alone: S 4096,
-// 32/8 heads of 128 262 / 260 / 259 us, with the polynomial 233 / 230 / 292; 16 heads of 64 133 / 133 / 132 and 119 / 116 / 146.
-// The coefficients take twelve registers, which is why the softmax keeps to exp2 beside a cap.
+// 32/8 heads of 128 262 / 260 / 259 us, with the polynomial 219 / 217 / 289; 16 heads of 64 133 / 133 / 132 and 113 / 110 / 145.
+// The coefficients take ten registers, which is why the softmax keeps to exp2 beside a cap.  They hold the powers of `in`, which
+// turns a raw score into x, so the polynomial is one of the raw score; where the ninth power would leave fp32 (or its product
+// with the cap its normal numbers), which no ordinary scale and cap do, every tile takes the formula.
 struct TanhPoly {
-  static constexpr float kLimit = 0.64f;  // of x^2
-  uint64_t in, c[5];
-  __device__ __forceinline__ TanhPoly(float in_scale, float cap) {
-    in = pack_f2(in_scale, in_scale);
+  float limit;  // of the square of a raw score
+  bool usable;
+  uint64_t c[5];
+  __device__ __forceinline__ TanhPoly(float in, float cap) {
+    usable = in > 2e-4f && in < 1e3f;
+    limit = 0.64f / (in * in);
+    float power = cap * in;
     const float k[5] = {0.9999951124191284f, -0.3331742584705353f, 0.13186223804950714f, -0.04826141893863678f,
                         0.011464733630418777f};
 #pragma unroll
-    for (int i = 0; i < 5; ++i) c[i] = pack_f2(cap * k[i], cap * k[i]);
+    for (int i = 0; i < 5; ++i, power *= in * in) c[i] = pack_f2(power * k[i], power * k[i]);
   }
-  // `top` follows the largest x^2
+  // `top` follows the largest square
   __device__ __forceinline__ uint64_t operator()(uint64_t score, uint64_t bias, float& top) const {
-    const uint64_t x = mul2(score, in);
-    const uint64_t u = mul2(x, x);
+    const uint64_t u = mul2(score, score);
     float u0, u1;
     unpack_f2(u, u0, u1);
     top = max3_nan(top, u0, u1);
@@ -88,15 +96,16 @@ struct TanhPoly {
     y = fma2(y, u, c[2]);
     y = fma2(y, u, c[1]);
     y = fma2(y, u, c[0]);
-    return fma2(x, y, bias);
+    return fma2(score, y, bias);
   }
 };
 
+template <int kKind>
 __device__ __forceinline__ void cap32(uint32_t (&r)[32], const TanhPoly& poly, uint64_t bias, uint64_t step, float& top) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     unpack_u2(poly(pack_u2(r[2 * i], r[2 * i + 1]), bias, top), r[2 * i], r[2 * i + 1]);
-    bias = add2(bias, step);
+    if (has_bias(kKind)) bias = add2(bias, step);
   }
 }
 
@@ -113,9 +122,10 @@ __device__ __forceinline__ float max32(const uint32_t (&r)[32]) {
 
 // Softmax warpgroups per query tile.  Where a CTA holds one tile only (head dim 256) and there is a cap, two of them share its
 // keys, half each, and compare their maxima: one alone has a warp per scheduler for all of the arithmetic.  S 4096, 16/8 heads of
-// 256, us, one and two: cap 181, 166; with a bias too 210, 189.  Without a cap one keeps up with the copies and the products, and
-// the comparing costs: 129, 132; with a bias 153, 153.
-constexpr int fwd_share(int NQ, int kind) { return NQ == 1 && kind == 2 ? 2 : 1; }
+// 256, us, one and two: cap 181, 166; with a bias too 210, 189 (before the polynomial became shorter).  Without a cap one keeps up with the
+// copies and the products, and the comparing costs: 129, 132; with a bias 153, 153.  With two tiles per CTA it loses, 104 registers
+// per thread being too few: 32/8 heads of 128 233, 284.
+constexpr int fwd_share(int NQ, int kind) { return NQ == 1 && has_cap(kind) ? 2 : 1; }
 constexpr int fwd_threads(int NQ, int kind) { return 128 + NQ * fwd_share(NQ, kind) * 128; }
 
 template <int DP, int BN, int NQ, int NS, typename T, int kKind>
@@ -128,7 +138,7 @@ __global__ void __launch_bounds__(fwd_threads(NQ, kKind), 1)
   constexpr int kPvParts = (DP == 64) ? 2 : 4;     // P is handed to the issuer in parts, as in the plain hop
   constexpr int kPartChunks = BN / 32 / kPvParts;
   constexpr int kShare = fwd_share(NQ, kKind);
-  constexpr int kPolyEvery = (NQ == 2 && kKind < 2) ? kFwdPolyEvery : 0;  // a cap keeps the FMA pipe busy
+  constexpr int kPolyEvery = (NQ == 2 && !has_cap(kKind)) ? kFwdPolyEvery : 0;  // a cap keeps the FMA pipe busy
 
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bar_q_full;
@@ -469,12 +479,12 @@ __global__ void __launch_bounds__(fwd_threads(NQ, kKind), 1)
       const Exp2Poly exp2_poly;
       const float scale_log2 = p.sc.scale * kLog2e;
       const float cap_log2 = p.sc.cap * kLog2e;
-      const float slope = kKind > 0 ? slope_log2(p.sc, b, p.Hq, h) : 0.f;
+      const float slope = has_bias(kKind) ? slope_log2(p.sc, b, p.Hq, h) : 0.f;
       const int ahead = p.sc.q_pos + row_g - p.sc.k_pos;  // position of this row, from the first key of the block
       // what a raw score is multiplied by, and the tanh's -2 cap
-      const float in_scale = kKind == 2 ? 2.f * scale_log2 / p.sc.cap : scale_log2;
+      const float in_scale = has_cap(kKind) ? 2.f * scale_log2 / p.sc.cap : scale_log2;
       const TanhPoly tanh_poly(p.sc.scale / p.sc.cap, cap_log2);
-      int direct = 0;  // tiles that take the formula at once
+      int direct = tanh_poly.usable ? 0 : INT_MAX;  // tiles that take the formula at once
       uint32_t pair_par = 0;
       // Waits for the other warp with these rows; what either wrote before, tensor memory included, the other sees after.
       auto pair_sync = [&]() {
@@ -526,17 +536,18 @@ __global__ void __launch_bounds__(fwd_threads(NQ, kKind), 1)
           // Keys all before or all after the queries: the distance is linear in the key, sign * (ahead - key).
           const int d0 = p.sc.q_pos + m0_q - p.sc.k_pos;  // of the first row
           const bool before = n0 + kKeys - 1 <= d0, after = n0 >= d0 + 127;
-          const bool linear = before || after || slope == 0.f;
+          const bool linear = !has_bias(kKind) || before || after || slope == 0.f;
           const float sign_slope = before ? slope : after ? -slope : 0.f;
           const uint64_t step = pack_f2(2.f * sign_slope, 2.f * sign_slope);
           const float first = static_cast<float>(n0 - ahead);  // minus the distance of the first key
           auto bias_of = [&](int c, float constant) {
+            if (!has_bias(kKind)) return pack_f2(constant, constant);
             const float b0 = fmaf(first + c * 32, sign_slope, constant);
             return pack_f2(b0, b0 + sign_slope);
           };
           auto formula_chunk = [&](int c) {
             transform32<kKind>(r[c], pack_f2(in_scale, in_scale), pack_f2(-2.f * cap_log2, -2.f * cap_log2),
-                               bias_of(c, kKind == 2 ? cap_log2 : 0.f), step);
+                               bias_of(c, has_cap(kKind) ? cap_log2 : 0.f), step);
           };
           auto formula = [&]() {
 #pragma unroll
@@ -553,11 +564,11 @@ __global__ void __launch_bounds__(fwd_threads(NQ, kKind), 1)
             }
             mask_and_max();
           };
-          if (kKind == 1 || direct > 0) {
+          if (!has_cap(kKind) || direct > 0) {
             formula();
             finish();
-            if (kKind == 2) --direct;
-          } else if constexpr (kKind == 2) {
+            if (has_cap(kKind)) --direct;
+          } else if constexpr (has_cap(kKind)) {
             // The polynomial first; chunks in which some lane left its range (garbage in masked places counts) are done again
             // from the scores, which are still in tensor memory.
             float top[NCH];
@@ -565,18 +576,18 @@ __global__ void __launch_bounds__(fwd_threads(NQ, kKind), 1)
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
               top[c] = 0.f;
-              cap32(r[c], tanh_poly, bias_of(c, 0.f), step, top[c]);
+              cap32<kKind>(r[c], tanh_poly, bias_of(c, 0.f), step, top[c]);
               mx = max_nan(mx, max32(r[c]));  // fills the gaps of the arithmetic; good where nothing changes any more
             }
             float most = top[0];
 #pragma unroll
             for (int c = 1; c < NCH; ++c) most = max_nan(most, top[c]);
-            const bool again = __any_sync(0xffffffffu, most > TanhPoly::kLimit);
+            const bool again = __any_sync(0xffffffffu, most > tanh_poly.limit);
             if (again) {
               int count = 0;
 #pragma unroll
               for (int c = 0; c < NCH; ++c)
-                if (__any_sync(0xffffffffu, top[c] > TanhPoly::kLimit)) {
+                if (__any_sync(0xffffffffu, top[c] > tanh_poly.limit)) {
                   tmem_ld32(s_addr + c * 32, r[c]);
                   tmem_ld_wait32(r[c]);
                   formula_chunk(c);
@@ -882,7 +893,9 @@ static int dispatch_scored_kind(const void* q, const void* k, const void* v, con
   switch (score_kind(prm.sc)) {
     case 0: return dispatch_scored_fwd<T, 0>(q, k, v, prm, dtype, stream);
     case 1: return dispatch_scored_fwd<T, 1>(q, k, v, prm, dtype, stream);
-    default: return dispatch_scored_fwd<T, 2>(q, k, v, prm, dtype, stream);
+    default:
+      return prm.sc.slopes ? dispatch_scored_fwd<T, 3>(q, k, v, prm, dtype, stream)
+                           : dispatch_scored_fwd<T, 2>(q, k, v, prm, dtype, stream);
   }
 }
 
