@@ -582,12 +582,13 @@ __global__ void __launch_bounds__(fwd_threads(NQ, kKind), 1)
             float most = top[0];
 #pragma unroll
             for (int c = 1; c < NCH; ++c) most = max_nan(most, top[c]);
-            const bool again = __any_sync(0xffffffffu, most > tanh_poly.limit);
+            // (a NaN, of padding or not, tells nothing about the others: the formula again)
+            const bool again = __any_sync(0xffffffffu, !(most <= tanh_poly.limit));
             if (again) {
               int count = 0;
 #pragma unroll
               for (int c = 0; c < NCH; ++c)
-                if (__any_sync(0xffffffffu, top[c] > tanh_poly.limit)) {
+                if (__any_sync(0xffffffffu, !(top[c] <= tanh_poly.limit))) {
                   tmem_ld32(s_addr + c * 32, r[c]);
                   tmem_ld_wait32(r[c]);
                   formula_chunk(c);

@@ -375,3 +375,18 @@ def test_no_number_reaches_its_row_from_any_share():
     bad[2000] = True
     assert torch.equal(out.isnan().all(-1).flatten(), bad) and torch.equal(out.isnan().any(-1).flatten(), bad)
     assert torch.equal(lse.isnan().flatten(), bad)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_scores_beyond_the_cap_beside_padding_that_is_no_number(D):
+    """Keys whose scores lie beyond the cap share a run of 32 keys with padding of NaN: their tanh is still exact."""
+    import opt_ring_flash_attn_b200 as rfa
+
+    S, end = 400, 330
+    q, k, v, dout = inputs(18, 1, S, 2, 1, D, BF, DEV)
+    k[0, end - 6:end] *= 30  # these only: a tile with many such scores would change the route of the next ones
+    ref = reference(q, k, v, dout, visible(S, False, [0, end], None, DEV), softcap=15.0)
+    mask = rfa.document_mask([0, end], S, causal=False, device=DEV)
+    for t in (q, k, v, dout):
+        t[:, end:] = math.nan
+    check(ref, **_run(q, k, v, dout, mask=mask, softcap=15.0))
