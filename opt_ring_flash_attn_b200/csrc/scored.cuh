@@ -107,9 +107,11 @@ inline int make_score_params(const rfa_score_args* a, int B, int S, ScoreParams*
   return RFA_OK;
 }
 
-// Kind of scores a kernel is instantiated for: 0 as they are, 1 with a distance bias, 2 capped (and, with slopes, biased).
-// Separate instantiations, because a bias costs a tile two operations per pair of scores and a cap several.
-inline int score_kind(const ScoreParams& s) { return s.cap > 0.f ? 2 : s.slopes ? 1 : 0; }
+// Kind of scores a kernel is instantiated for: 0 as they are, 1 with a distance bias, 2 capped, 3 both.  Separate
+// instantiations, because a bias costs a tile two operations per pair of scores and a cap several.
+inline int score_kind(const ScoreParams& s) { return (s.cap > 0.f ? 2 : 0) + (s.slopes ? 1 : 0); }
+__host__ __device__ constexpr bool has_cap(int kind) { return kind >= 2; }
+__host__ __device__ constexpr bool has_bias(int kind) { return kind % 2 == 1; }
 
 __device__ __forceinline__ float slope_log2(const ScoreParams& s, int b, int Hq, int h) {
   return s.slopes ? __ldg(s.slopes + (s.slopes_per_batch ? static_cast<size_t>(b) * Hq : 0) + h) * kLog2e : 0.f;

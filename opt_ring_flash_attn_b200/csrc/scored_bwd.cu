@@ -15,7 +15,8 @@
 //
 // Bound, as the plain hop, by the serial order of a tile's steps (tensor pipe 52 % busy with documents, 34 % at head dim 64);
 // with a cap by the elementwise warps, which issue some fourteen instructions more per pair.  Whole backward pass, causal, us:
-// S 4096, 32/8 heads of 128: no change 391, bias 393, cap 499; 16 heads of 64: 160, 167, 230; 16/8 heads of 256: 560, 553, 578.
+// S 4096, 32/8 heads of 128: no change 391, bias 392, cap 471, both 502; 16 heads of 64: 158, 165, 218, 228; 16/8 heads of 256: 560, 550, 570,
+// 570.  (A cap with a running bias of 0 instead of an instantiation of its own: 499, 230, 578.)
 // Taking the tile coordinates out of registers (BwdPlan) was worth 12 to 20 %: 199 -> 159 us (16 heads of 64 with a bias).  A
 // polynomial for the tanh, as in the forward hop, loses here: 517 -> 556 us; the special-function unit is not what binds.
 // dQ and dK carry three roundings to 16 bits: W, dX and the result (and delta that of out).
@@ -517,7 +518,7 @@ __global__ void __launch_bounds__(640, 1)
     const uint32_t a_dp = tmem_base + lane_addr + Cfg::kTmDP + col0;
     const uint64_t nscale2 = pack_f2(-p.scale_log2, -p.scale_log2);
     const float cap_log2 = sc.cap * kLog2e;
-    const float in_scale = kKind == 2 ? 2.f * p.scale_log2 / sc.cap : 0.f;  // raw score to the exponent of the tanh
+    const float in_scale = has_cap(kKind) ? 2.f * p.scale_log2 / sc.cap : 0.f;  // raw score to the exponent of the tanh
     const int ahead = sc.q_pos + col0 - (sc.k_pos + kvpos);  // of query column col0 of tile 0 over this key
     bool ok = run;
     if (Cfg::kKTmem && run) {
@@ -560,9 +561,9 @@ __global__ void __launch_bounds__(640, 1)
         for (int c = 1; c < NCH; ++c) reg_fence32(r[c]);
         // P^T = exp2(z - lse2) = exp2(-y); the distance term slope |i - j| is linear in the query where all queries of the
         // tile lie on one side of all keys.
-        const float slope = kKind > 0 ? slope_log2(sc, b, p.Hq, walk.head(t)) : 0.f;
+        const float slope = has_bias(kKind) ? slope_log2(sc, b, p.Hq, walk.head(t)) : 0.f;
         const int d0 = sc.q_pos + i * BQ - (sc.k_pos + n0);  // of the first query over the first key
-        const bool linear = d0 >= 127 || d0 + BQ - 1 <= 0 || slope == 0.f;
+        const bool linear = !has_bias(kKind) || d0 >= 127 || d0 + BQ - 1 <= 0 || slope == 0.f;
         const float sign_slope = d0 >= 127 ? slope : -slope;
         auto p_phase = [&](auto mask_tag, auto linear_tag) {
           constexpr bool kMask = decltype(mask_tag)::value;
@@ -575,8 +576,8 @@ __global__ void __launch_bounds__(640, 1)
             uint64_t bias = 0;
             if (kKind > 0) {
               // what y has beside lse2: the distance and the constant of the tanh
-              const float b0 = (kLinear ? static_cast<float>(d) * sign_slope : 0.f) - (kKind == 2 ? cap_log2 : 0.f);
-              bias = pack_f2(b0, kLinear ? b0 + sign_slope : b0);
+              const float b0 = (has_bias(kKind) && kLinear ? static_cast<float>(d) * sign_slope : 0.f) - (has_cap(kKind) ? cap_log2 : 0.f);
+              bias = pack_f2(b0, has_bias(kKind) && kLinear ? b0 + sign_slope : b0);
             }
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
@@ -584,11 +585,11 @@ __global__ void __launch_bounds__(640, 1)
               uint64_t y2 = pack_f2(l2.x, l2.y);
               if (kKind > 0) {
                 y2 = add2(y2, bias);
-                if (kLinear) bias = add2(bias, step);
-                else y2 = add2(y2, pack_f2(slope * fabsf(static_cast<float>(d + 2 * k)), slope * fabsf(static_cast<float>(d + 2 * k + 1))));
+                if (has_bias(kKind) && kLinear) bias = add2(bias, step);
+                else if (has_bias(kKind)) y2 = add2(y2, pack_f2(slope * fabsf(static_cast<float>(d + 2 * k)), slope * fabsf(static_cast<float>(d + 2 * k + 1))));
               }
               uint64_t jac2 = 0;
-              if constexpr (kKind == 2) {
+              if constexpr (has_cap(kKind)) {
                 // cap tanh(x / cap) = cap - cap g and 1 - tanh^2 = g (2 - g) with g = 2 / (exp(2 x / cap) + 1)
                 float a0, a1;
                 unpack_f2(mul2(pack_u2(r[c][2 * k], r[c][2 * k + 1]), pack_f2(in_scale, in_scale)), a0, a1);
@@ -609,7 +610,7 @@ __global__ void __launch_bounds__(640, 1)
                 if (static_cast<unsigned>(qp + 1) >= static_cast<unsigned>(width)) e1 = 0.f;
               }
               u[k] = Pack2<T>::pack(e0, e1);
-              if constexpr (kKind == 2) {
+              if constexpr (has_cap(kKind)) {
                 float w0, w1;
                 unpack_f2(mul2(pack_f2(e0, e1), jac2), w0, w1);
                 pk[c * 16 + k] = Pack2<T>::pack(w0, w1);
@@ -621,7 +622,7 @@ __global__ void __launch_bounds__(640, 1)
             tmem_st16(a_s + c * 16, u);
           }
         };
-        if (kKind > 0 && !linear) {
+        if (has_bias(kKind) && !linear) {
           if (masked) p_phase(std::true_type{}, std::false_type{});
           else p_phase(std::false_type{}, std::false_type{});
         } else {
@@ -912,7 +913,8 @@ static int dispatch_kind(const void* q, const void* k, const void* v, const void
   switch (score_kind(prm.sc)) {
     case 0: return dispatch_dim<T, 0>(q, k, v, dout, prm, dtype, stream);
     case 1: return dispatch_dim<T, 1>(q, k, v, dout, prm, dtype, stream);
-    default: return dispatch_dim<T, 2>(q, k, v, dout, prm, dtype, stream);
+    case 2: return dispatch_dim<T, 2>(q, k, v, dout, prm, dtype, stream);
+    default: return dispatch_dim<T, 3>(q, k, v, dout, prm, dtype, stream);
   }
 }
 

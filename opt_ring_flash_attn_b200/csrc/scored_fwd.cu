@@ -38,10 +38,6 @@ struct ScoredFwdParams {
   ScoreParams sc;
 };
 
-// What happens to the scores, as the kernels are instantiated: 0 nothing, 1 a bias, 2 a cap, 3 both.
-constexpr bool has_cap(int kind) { return kind >= 2; }
-constexpr bool has_bias(int kind) { return kind % 2 == 1; }
-
 // Scores of 32 keys in log2 units: the cap and the bias.  `bias` holds what is added to the first two keys, `step` what it
 // grows by from pair to pair (bias and step include the constant of the tanh).
 template <int kKind>
@@ -894,9 +890,8 @@ static int dispatch_scored_kind(const void* q, const void* k, const void* v, con
   switch (score_kind(prm.sc)) {
     case 0: return dispatch_scored_fwd<T, 0>(q, k, v, prm, dtype, stream);
     case 1: return dispatch_scored_fwd<T, 1>(q, k, v, prm, dtype, stream);
-    default:
-      return prm.sc.slopes ? dispatch_scored_fwd<T, 3>(q, k, v, prm, dtype, stream)
-                           : dispatch_scored_fwd<T, 2>(q, k, v, prm, dtype, stream);
+    case 2: return dispatch_scored_fwd<T, 2>(q, k, v, prm, dtype, stream);
+    default: return dispatch_scored_fwd<T, 3>(q, k, v, prm, dtype, stream);
   }
 }
 
