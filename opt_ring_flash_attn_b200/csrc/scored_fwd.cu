@@ -16,7 +16,7 @@
 // Bound, as the plain hop, by the chain of one query tile (scores, softmax, products), which two tiles per CTA overlap; by the
 // start and end of CTAs where documents are short (5 us of a CTA's 30 at 13 key tiles a pair); and with a cap by the arithmetic
 // units, whose phases (cap, maximum, exponentials) one warpgroup goes through in turn.  Forward hop, causal, us: S 4096, 32/8
-// heads of 128: no change 140, bias 175, cap 219, both 245; 16 heads of 64: 64, 77, 113, 123; 16/8 heads of 256: 129, 153, 157, 187.
+// heads of 128: no change 132, bias 173, cap 195, both 232; 16 heads of 64: 63, 77, 98, 118; 16/8 heads of 256: 122, 153, 154, 186.
 // S 16384, 32/8 heads of 128, ten documents: 422 us = 832 TFLOP/s of visible pairs, tensor pipe 48 % busy.
 #include "fwd_common.cuh"
 #include "scored.cuh"
@@ -65,7 +65,8 @@ __device__ __forceinline__ void transform32(uint32_t (&r)[32], uint64_t scale2, 
 // to even out the absolute error of the tanh: 3.5e-7).  The formula with exp2 and a reciprocal takes two turns on the
 // special-function unit per score, beside the one of the softmax, which makes it the unit that a tile waits for.  Forward hop,
 // scores of 3.2 on average, caps of 50 / 20 / 5 (where no, few and most chunks leave the range), by the formula alone: S 4096,
-// 32/8 heads of 128 262 / 260 / 259 us, with the polynomial 219 / 217 / 289; 16 heads of 64 133 / 133 / 132 and 113 / 110 / 145.
+// 32/8 heads of 128 262 / 260 / 259 us, with the polynomial 219 / 217 / 289; 16 heads of 64 133 / 133 / 132 and 113 / 110 / 145
+// (before the masks became cheaper).
 // The coefficients take ten registers, which is why the softmax keeps to exp2 beside a cap.  They hold the powers of `in`, which
 // turns a raw score into x, so the polynomial is one of the raw score; where the ninth power would leave fp32 (or its product
 // with the cap its normal numbers), which no ordinary scale and cap do, every tile takes the formula.
@@ -104,6 +105,9 @@ __device__ __forceinline__ void cap32(uint32_t (&r)[32], const TanhPoly& poly, u
     if (has_bias(kKind)) bias = add2(bias, step);
   }
 }
+
+// The lowest n of 32 bits; none for n < 0, all for n > 32.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1u; }
 
 // Largest of 32 scores (independent partial maxima keep the dependency chains short).
 __device__ __forceinline__ float max32(const uint32_t (&r)[32]) {
@@ -514,13 +518,18 @@ __global__ void __launch_bounds__(fwd_threads(NQ, kKind), 1)
         float mx;
         auto mask_and_max = [&]() {
           if (masked) {
-            const int base = n0 - lo;
+            // One word of bits per 32 keys, and nothing for those that the whole warp sees: beside a compare per key and row,
+            // S 16384, documents of 2048, 32/8 heads of 128: no change 347 -> 340 us, cap 525 -> 485, both 606 -> 572.
 #pragma unroll
-            for (int c = 0; c < NCH; ++c)
+            for (int c = 0; c < NCH; ++c) {
+              const int from = lo - (n0 + c * 32);
+              const uint32_t seen = low_bits(from + width) & ~low_bits(from);
+              if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (static_cast<unsigned>(base + c * 32 + i) >= static_cast<unsigned>(width))
-                  r[c][i] = __float_as_uint(-INFINITY);
+                for (int i = 0; i < 32; ++i)
+                  if (!(seen >> i & 1u)) r[c][i] = __float_as_uint(-INFINITY);
+              }
+            }
           }
           mx = max32(r[0]);
 #pragma unroll
@@ -529,9 +538,10 @@ __global__ void __launch_bounds__(fwd_threads(NQ, kKind), 1)
         if constexpr (kKind == 0) {
           mask_and_max();
         } else {
-          // Keys all before or all after the queries: the distance is linear in the key, sign * (ahead - key).
-          const int d0 = p.sc.q_pos + m0_q - p.sc.k_pos;  // of the first row
-          const bool before = n0 + kKeys - 1 <= d0, after = n0 >= d0 + 127;
+          // Keys all before or all after the warp's queries: the distance is linear in the key, sign * (ahead - key).  (To tell
+          // that apart for every 32 keys of a tile costs more than it saves: 77 us for 76, S 4096, 16 heads of 64 with a bias.)
+          const int d0 = p.sc.q_pos + m0_q + quarter * 32 - p.sc.k_pos;  // of the warp's first row
+          const bool before = n0 + kKeys - 1 <= d0, after = n0 >= d0 + 31;
           const bool linear = !has_bias(kKind) || before || after || slope == 0.f;
           const float sign_slope = before ? slope : after ? -slope : 0.f;
           const uint64_t step = pack_f2(2.f * sign_slope, 2.f * sign_slope);
