@@ -15,7 +15,7 @@
 //
 // Bound, as the plain hop, by the chain of one query tile (scores, softmax, products), which two tiles per CTA overlap; by the
 // start and end of CTAs where documents are short (5 us of a CTA's 30 at 13 key tiles a pair); and with a cap by the arithmetic
-// units, whose phases (cap, maximum, exponentials) one warpgroup goes through in turn.  Forward hop, causal, us: S 4096, 32/8
+// units, whose phases (cap, maximum, exponentials) a warpgroup goes through in turn.  Forward hop, causal, us: S 4096, 32/8
 // heads of 128: no change 132, bias 173, cap 195, both 232; 16 heads of 64: 63, 77, 98, 118; 16/8 heads of 256: 122, 153, 154, 186.
 // S 16384, 32/8 heads of 128, ten documents: 422 us = 832 TFLOP/s of visible pairs, tensor pipe 48 % busy.
 #include "fwd_common.cuh"
