@@ -260,9 +260,19 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(T* __restrict__ k, T* _
 // instructions instead of 42.)
 //   q enters as fp16, each row under a power of two and the channels of odd codes under 2^-4 of it: exact for fp16 and bf16.
 //   The minima meet the group sums of q, split in two 16-bit parts, in one more product with the meta words as they are.
-//   P sc is rounded to fp16 (11 bits, for bf16 caches too), under a power of two that keeps it in range.  For fp16 results
-//   u - 8 stands in for u, which halves what that rounding weighs (min + 8 sc makes up for it): relative error of fp16
+//   P sc is rounded to fp16 (11 bits, for bf16 caches too), under a power of two per group of 32 channels that brings the
+//   largest scale of V that the run has met to 2^4 or more (weights are 4 at most).  So P sc loses bits where it is less than 2^-18 of the
+//   group's largest scale, at most 2^-29 of that scale a token.  (One power for all groups took the bits from the small ones: beside
+//   a group 2^17 times as large, results were off by 7 %.)  The powers lie in shared memory: in registers, which the kernel has none
+//   to spare of, b64 below takes 97 us, with one power for all 92.
+//   For fp16 results u - 8 stands in for u, which halves what that rounding weighs (min + 8 sc makes up for it): relative error of fp16
 //   results 2.8e-4 instead of 4.8e-4, where rounding the result alone gives 2.1e-4.
+constexpr float kMostDown = 2.6584559915698317e36f;  // 2^121, what scales of V are multiplied with before any was seen
+constexpr float kDownLimit = 4096.f;                 // of a scale times its power: with weights up to 2^2 far inside fp16
+
+// 1 / x of a power of two in [2^-126, 2^126].
+__device__ __forceinline__ float power_rcp(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
+
 struct Kv4AttnParams {
   const void* q;
   const uint8_t* codes;
@@ -497,6 +507,7 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
   __shared__ uint64_t bar_full[2][kRing], bar_empty[2][kRing];
   __shared__ int page_ok[2][kRing];
   __shared__ Kv4Fetch fetcher[2];
+  __shared__ __align__(16) float v_down_s[4][NG];  // powers of two on the scales of V, per warp and group of channels
   __shared__ int abort_flag, skip_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -636,7 +647,9 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
       }
     }
     float o[NT][NG][2][4], corr[NT][NG][2], m[NT][2], l[NT][2];
-    float v_down = 1.f, v_limit = 0.f;  // power of two on the scales of V, and the largest scale it is good for
+    __syncwarp();
+    if (lane < NG) v_down_s[warp][lane] = kMostDown;
+    __syncwarp();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -804,51 +817,51 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
               if (far + j * 16 + rt + 8 >= there) e1[g] = 0;
             }
           }
-          float sc0[NG], sc1[NG], most = 0.f;
+          float sc0[NG], sc1[NG], most = 0.f, v_down[NG];
+          lds_words<NG>(reinterpret_cast<uint32_t(&)[NG]>(v_down), reinterpret_cast<const uint8_t*>(v_down_s[warp]));
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            sc0[g] = Kv4Type<T>::lo(e0[g]);
-            sc1[g] = Kv4Type<T>::lo(e1[g]);
-            most = fmaxf(fmaxf(most, sc0[g]), sc1[g]);
+            sc0[g] = Kv4Type<T>::lo(e0[g]) * v_down[g];
+            sc1[g] = Kv4Type<T>::lo(e1[g]) * v_down[g];
+            most = fmaxf(fmaxf(most, fabsf(sc0[g])), fabsf(sc1[g]));
           }
-          if (__any_sync(0xffffffffu, most > v_limit && most < INFINITY)) {
-            // the first scales, or 2^8 above those the power was chosen for: it is chosen again, the largest comes to [1, 2)
-            if (!(most < INFINITY)) most = 0.f;
+          if (__any_sync(0xffffffffu, most > kDownLimit)) {
+            // A group whose scales outgrew their power, as the first ones do (or that holds no number: it tells nothing about
+            // the others, and changes nothing): the power is chosen again, the largest of the group comes to [2^4, 2^5).
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-            const int ex = min(max(static_cast<int>(__float_as_uint(most) >> 23), 10), 245);
-            const float down = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
-            const float f = down / v_down;
-            v_down = down;
-            v_limit = __uint_as_float(static_cast<uint32_t>(min(ex + 8, 254)) << 23);
+            for (int g = 0; g < NG; ++g) {
+              const float a = fabsf(Kv4Type<T>::lo(e0[g])), b = fabsf(Kv4Type<T>::lo(e1[g]));
+              const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(a < INFINITY ? a : 0.f, b < INFINITY ? b : 0.f)));
+              const bool change = __uint_as_float(top) * v_down[g] > kDownLimit;
+              const float down = change ? __uint_as_float((258u - (top >> 23)) << 23) : v_down[g];
+              const float f = down * power_rcp(v_down[g]);
+              v_down[g] = down;
+              if (lane == 0) v_down_s[warp][g] = down;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int g = 0; g < NG; ++g)
+              for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                   o[nt][g][0][x] *= f;
                   o[nt][g][1][x] *= f;
                 }
+              sc0[g] = Kv4Type<T>::lo(e0[g]) * v_down[g];
+              sc1[g] = Kv4Type<T>::lo(e1[g]) * v_down[g];
+            }
+            __syncwarp();
           }
-          float pd[NT][4];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) pd[nt][x] = s[j][nt][x] * v_down;
           // P sc as the B operand, in fp16
           uint32_t pb[NT][NG][2];
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             float mn0 = Kv4Type<T>::hi(e0[g]), mn1 = Kv4Type<T>::hi(e1[g]);
             if (kCentred) {
-              mn0 = fmaf(8.f, sc0[g], mn0);
-              mn1 = fmaf(8.f, sc1[g], mn1);
+              mn0 = fmaf(8.f, Kv4Type<T>::lo(e0[g]), mn0);
+              mn1 = fmaf(8.f, Kv4Type<T>::lo(e1[g]), mn1);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              pb[nt][g][0] = transpose8x8(Pack2<__half>::pack(pd[nt][0] * sc0[g], pd[nt][1] * sc0[g]));
-              pb[nt][g][1] = transpose8x8(Pack2<__half>::pack(pd[nt][2] * sc1[g], pd[nt][3] * sc1[g]));
+              pb[nt][g][0] = transpose8x8(Pack2<__half>::pack(s[j][nt][0] * sc0[g], s[j][nt][1] * sc0[g]));
+              pb[nt][g][1] = transpose8x8(Pack2<__half>::pack(s[j][nt][2] * sc1[g], s[j][nt][3] * sc1[g]));
               corr[nt][g][0] = fmaf(s[j][nt][0], mn0, fmaf(s[j][nt][2], mn1, corr[nt][g][0]));
               corr[nt][g][1] = fmaf(s[j][nt][1], mn0, fmaf(s[j][nt][3], mn1, corr[nt][g][1]));
             }
@@ -886,7 +899,6 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
     // ---- the four warps' results of this run into one ----
     float* join = reinterpret_cast<float*>(smem + Cfg::kOffJoin);
     float* ml = reinterpret_cast<float*>(smem + Cfg::kOffMl);
-    const float v_up = 1.f / v_down * 1048576.f;  // 2^20 of the odd codes; the even ones carry 2^4 more
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -923,13 +935,15 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
           for (int x = 0; x < 2; ++x) {
             const float f = fast_exp2(m[nt][x] - top[nt][x]);
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {  // channels 32 g + 4 r + (0..3)
+            for (int g = 0; g < NG; ++g) {  // channels 32 g + 4 r + (0..3); even codes carry 2^24, odd ones 2^20
+              const float up = f * power_rcp(v_down_s[warp][g]);
               float4* dst = reinterpret_cast<float4*>(join + (pair * kRows + nt * 8 + 2 * c + x) * D + g * kGroup + 4 * r);
               const float4 old = w == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *dst;
-              *dst = make_float4(fmaf(fmaf(o[nt][g][0][x], 16.f * v_up, corr[nt][g][x]), f, old.x),
-                                 fmaf(fmaf(o[nt][g][0][x + 2], v_up, corr[nt][g][x]), f, old.y),
-                                 fmaf(fmaf(o[nt][g][1][x], 16.f * v_up, corr[nt][g][x]), f, old.z),
-                                 fmaf(fmaf(o[nt][g][1][x + 2], v_up, corr[nt][g][x]), f, old.w));
+              const float rest = corr[nt][g][x] * f;
+              *dst = make_float4(fmaf(o[nt][g][0][x] * 16777216.f, up, rest) + old.x,
+                                 fmaf(o[nt][g][0][x + 2] * 1048576.f, up, rest) + old.y,
+                                 fmaf(o[nt][g][1][x] * 16777216.f, up, rest) + old.z,
+                                 fmaf(o[nt][g][1][x + 2] * 1048576.f, up, rest) + old.w);
             }
           }
       }
