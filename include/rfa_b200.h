@@ -316,6 +316,14 @@ int rfa_kv4_attn(const void* q, const long long* q_strides, const void* codes, c
                  const int* table, int max_pages, const int* lens, void* out, float* lse, float* scratch, int B, int T, int Hq,
                  int Hkv, int D, int dtype, float softmax_scale, float softcap, const float* slopes, int slopes_per_batch,
                  int* status, void* stream);
+/* The same over a part of each sequence's tokens, the others lying in other caches: after[b] (int32 [B], device memory, or NULL:
+ * none; negative ones are 0) tokens follow those of this one, so that token t of q is at position lens[b] + after[b] - T + t counted from this part's
+ * first; it sees the keys up to itself, at distances counted from there.  out and lse of the parts, joined by their lse, are
+ * those of the whole. */
+int rfa_kv4_attn_part(const void* q, const long long* q_strides, const void* codes, const void* meta, int n_pages,
+                      const int* table, int max_pages, const int* lens, const int* after, void* out, float* lse,
+                      float* scratch, int B, int T, int Hq, int Hkv, int D, int dtype, float softmax_scale, float softcap,
+                      const float* slopes, int slopes_per_batch, int* status, void* stream);
 
 /*
  * Packs K and V ([B, Skv, Hkv, D] each, `bytes_each` bytes) into one contiguous

@@ -60,6 +60,7 @@ SIGNATURES = {
     "rfa_kv4_append": (_i, [_vp] * 6 + [_i, _vp, _i] + [_vp] * 2 + [_i] * 5 + [_vp]),
     "rfa_kv4_gather": (_i, [_vp] * 4 + [_i, _vp, _i] + [_vp] * 2 + [_i] * 5 + [_vp]),
     "rfa_kv4_attn": (_i, [_vp] * 4 + [_i, _vp, _i] + [_vp] * 4 + [_i] * 6 + [_f] * 2 + [_vp, _i] + [_vp] * 2),
+    "rfa_kv4_attn_part": (_i, [_vp] * 4 + [_i, _vp, _i] + [_vp] * 5 + [_i] * 6 + [_f] * 2 + [_vp, _i] + [_vp] * 2),
     "rfa_noalloc_scratch_bytes": (_sz, []),
     "rfa_bwd_hop_noalloc": (_i, [_vp] * 9 + [_i] * 7 + [_f] + [_i] * 2 + [_vp, _vp]),
     "rfa_dkdv_accumulate": (_i, [_vp, _vp, _vp, _sz, _vp]),
@@ -367,16 +368,16 @@ def kv4_scratch_elems(B: int, T: int, Hq: int, Hkv: int, D: int) -> int:
     return n
 
 
-def kv4_attn(q, codes, meta, table, lens, out, lse, scratch, softmax_scale: float, softcap: float, slopes, status,
+def kv4_attn(q, codes, meta, table, lens, after, out, lse, scratch, softmax_scale: float, softcap: float, slopes, status,
              stream=None) -> None:
     B, T, Hq, D = q.shape
     with _on_device(q):
-        rc = load().rfa_kv4_attn(q.data_ptr(), _strides(q), codes.data_ptr(), meta.data_ptr(), codes.shape[0],
-                                 table.data_ptr(), table.shape[1], lens.data_ptr(), out.data_ptr(), _ptr(lse),
-                                 scratch.data_ptr(), B, T, Hq, codes.shape[1], D, DTYPE_CODES[q.dtype], softmax_scale,
-                                 softcap, _ptr(slopes), int(slopes is not None and slopes.dim() == 2), status.data_ptr(),
-                                 _stream(stream, q))
-    _check(rc, "rfa_kv4_attn", kernels=2)
+        rc = load().rfa_kv4_attn_part(q.data_ptr(), _strides(q), codes.data_ptr(), meta.data_ptr(), codes.shape[0],
+                                      table.data_ptr(), table.shape[1], lens.data_ptr(), _ptr(after), out.data_ptr(),
+                                      _ptr(lse), scratch.data_ptr(), B, T, Hq, codes.shape[1], D, DTYPE_CODES[q.dtype],
+                                      softmax_scale, softcap, _ptr(slopes), int(slopes is not None and slopes.dim() == 2),
+                                      status.data_ptr(), _stream(stream, q))
+    _check(rc, "rfa_kv4_attn_part", kernels=2)
 
 
 def bwd_hop_noalloc(q, k, v, dout, lse2, delta, dq, dkdv_prev, dkdv_out, softmax_scale: float,

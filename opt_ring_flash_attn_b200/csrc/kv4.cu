@@ -279,6 +279,7 @@ struct Kv4AttnParams {
   const void* meta;
   const int* table;
   const int* lens;
+  const int* after;  // [B] or null: tokens of each sequence that lie behind those of this cache, in other parts of it
   void* out;
   float* lse;
   float* part_o;   // [2 * blocks][rows][D]
@@ -507,7 +508,8 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
   __shared__ uint64_t bar_full[2][kRing], bar_empty[2][kRing];
   __shared__ int page_ok[2][kRing];
   __shared__ Kv4Fetch fetcher[2];
-  __shared__ __align__(16) float v_down_s[4][NG];  // powers of two on the scales of V, per warp and group of channels
+  // per warp, in shared memory because registers are short: powers of two on the scales of V per group, slopes per column
+  __shared__ __align__(16) float v_down_s[4][NG], slope_s[4][8 * NT];
   __shared__ int abort_flag, skip_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -587,10 +589,12 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
       continue;
     }
     const int head = at.u / n_row_tiles, row0 = at.u % n_row_tiles * kRows;
+    __syncwarp();  // the last run's slopes and powers have been read
     // Query rows as the B operand: this lane holds channels [32 g + 8 c, + 8) of row r of each column tile.
     uint32_t qf[NT][NG][4], qs[NT][kQuads][2];
-    float zs[NT][2], slope[NT][2];
-    int lim[NT][2];  // last key that the row sees
+    float zs[NT][2];
+    int lim[NT][2];  // position of the row, the last that it sees (in another part of the cache, where tokens lie behind this one)
+    const int end = at.len + (p.after ? min(max(__ldg(p.after + at.b), 0), INT_MAX - at.len) : 0);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = row0 + nt * 8 + (kHalf ? r & 3 : r);
@@ -640,14 +644,12 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
       for (int i = 0; i < 2; ++i) {
         const int col = row0 + nt * 8 + (kHalf ? (2 * c + i) & 3 : 2 * c + i);
         zs[nt][i] = __shfl_sync(0xffffffffu, back, (2 * c + i) * 4) * (p.cap_log2 > 0.f ? p.cap_in : p.scale_log2);
-        lim[nt][i] = col < n_rows ? at.len - p.T + col / G : -1;
-        slope[nt][i] = 0.f;
-        if (p.slopes && col < n_rows)
-          slope[nt][i] = __ldg(p.slopes + (p.slopes_per_batch ? static_cast<size_t>(at.b) * p.Hq : 0) + head * G + col % G) * kLog2e;
+        lim[nt][i] = col < n_rows ? end - p.T + col / G : -1;
+        if (p.slopes && r == 0)
+          slope_s[warp][nt * 8 + 2 * c + i] = col < n_rows ? __ldg(p.slopes + (p.slopes_per_batch ? static_cast<size_t>(at.b) * p.Hq : 0) + head * G + col % G) * kLog2e : 0.f;
       }
     }
     float o[NT][NG][2][4], corr[NT][NG][2], m[NT][2], l[NT][2];
-    __syncwarp();
     if (lane < NG) v_down_s[warp][lane] = kMostDown;
     __syncwarp();
 #pragma unroll
@@ -745,22 +747,23 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
+              const float slope = slope_s[warp][nt * 8 + 2 * c + x];
               const float ahead = static_cast<float>(lim[nt][x] - (pos0 + far + rt));  // of the row over its first key here
 #pragma unroll
               for (int j = 0; j < kJ; ++j) {
-                s[j][nt][x] = fmaf(-slope[nt][x], ahead - 16.f * j, s[j][nt][x]);
-                s[j][nt][x + 2] = fmaf(-slope[nt][x], ahead - (16.f * j + 8.f), s[j][nt][x + 2]);
+                s[j][nt][x] = fmaf(-slope, ahead - 16.f * j, s[j][nt][x]);
+                s[j][nt][x + 2] = fmaf(-slope, ahead - (16.f * j + 8.f), s[j][nt][x + 2]);
               }
             }
         }
-        if (pos0 + 31 > at.len - p.T) {  // some row does not see all of them
+        if (there < 31 + p.T) {  // some row may not see all of them
 #pragma unroll
           for (int j = 0; j < kJ; ++j)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int x = 0; x < 4; ++x)
-                if (pos0 + far + j * 16 + rt + (x < 2 ? 0 : 8) > lim[nt][x & 1]) s[j][nt][x] = -INFINITY;
+                if (far + j * 16 + rt + (x < 2 ? 0 : 8) > min(lim[nt][x & 1] - pos0, there - 1)) s[j][nt][x] = -INFINITY;
         }
         // ---- running maximum: it follows when a score is more than 2^2 above it, or is no number ----
         bool grow = false;
@@ -1209,6 +1212,14 @@ extern "C" int rfa_kv4_attn(const void* q, const long long* q_strides, const voi
                             const int* table, int max_pages, const int* lens, void* out, float* lse, float* scratch, int B,
                             int T, int Hq, int Hkv, int D, int dtype, float softmax_scale, float softcap, const float* slopes,
                             int slopes_per_batch, int* status, void* stream) {
+  return rfa_kv4_attn_part(q, q_strides, codes, meta, n_pages, table, max_pages, lens, nullptr, out, lse, scratch, B, T, Hq, Hkv,
+                           D, dtype, softmax_scale, softcap, slopes, slopes_per_batch, status, stream);
+}
+
+extern "C" int rfa_kv4_attn_part(const void* q, const long long* q_strides, const void* codes, const void* meta, int n_pages,
+                                 const int* table, int max_pages, const int* lens, const int* after, void* out, float* lse,
+                                 float* scratch, int B, int T, int Hq, int Hkv, int D, int dtype, float softmax_scale,
+                                 float softcap, const float* slopes, int slopes_per_batch, int* status, void* stream) {
   using namespace rfa;
   if (!q || !q_strides || !out || !scratch || !status) return RFA_ERR_INVALID_ARG;
   const int rc = kv4_check(codes, meta, n_pages, table, max_pages, lens, B, T, Hkv, D, dtype);
@@ -1220,7 +1231,7 @@ extern "C" int rfa_kv4_attn(const void* q, const long long* q_strides, const voi
     if (q_strides[i] % 8 != 0) return RFA_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(q) & 15u) || (reinterpret_cast<uintptr_t>(out) & 15u) ||
       (reinterpret_cast<uintptr_t>(scratch) & 15u) || (reinterpret_cast<uintptr_t>(lse) & 3u) ||
-      (reinterpret_cast<uintptr_t>(slopes) & 3u))
+      (reinterpret_cast<uintptr_t>(slopes) & 3u) || (reinterpret_cast<uintptr_t>(after) & 3u))
     return RFA_ERR_INVALID_ARG;
   const int nt = kv4_tiles(T, Hq / Hkv, D), rows = 8 * nt;
   const long long row_tiles = (static_cast<long long>(T) * (Hq / Hkv) + rows - 1) / rows;
@@ -1232,6 +1243,7 @@ extern "C" int rfa_kv4_attn(const void* q, const long long* q_strides, const voi
   p.meta = meta;
   p.table = table;
   p.lens = lens;
+  p.after = after;
   p.out = out;
   p.lse = lse;
   p.q_b = q_strides[0];

@@ -136,13 +136,14 @@ def kv4_gather(cache: KV4Cache, block_table: torch.Tensor, positions: torch.Tens
     return k, v
 
 
-def _attn(q, cache, block_table, lens, softmax_scale, softcap, alibi_slopes, want_lse):
+def _attn(q, cache, block_table, lens, softmax_scale, softcap, alibi_slopes, want_lse, tokens_after=None):
     _check_tokens(q, cache, None, "q")
     B, T, Hq, D = q.shape
     if Hq == 0 or Hq % cache.n_kv_heads != 0:
         raise ValueError(f"H_q must be a multiple of the cache's {cache.n_kv_heads} heads, got {Hq}")
     table = _check_ints(block_table, B, cache.device, "block_table", 2)
     lens = _check_ints(lens, B, cache.device, "lens")
+    after = _check_ints(tokens_after, B, cache.device, "tokens_after")
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not (scale > 0) or math.isinf(scale):
         raise ValueError("softmax_scale must be positive and finite")
@@ -160,8 +161,8 @@ def _attn(q, cache, block_table, lens, softmax_scale, softcap, alibi_slopes, wan
     lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if want_lse else None
     # scratch per call: calls on several streams, or in several captured graphs, do not meet in it
     scratch = torch.empty(_native.kv4_scratch_elems(B, T, Hq, cache.n_kv_heads, D), dtype=torch.float32, device=q.device)
-    _native.kv4_attn(_rows(q), cache.codes, cache.meta, table, lens, out, lse, scratch, scale, softcap, slopes,
-                     ws.status)
+    _native.kv4_attn(_rows(q), cache.codes, cache.meta, table, lens, after, out, lse, scratch, scale, softcap,
+                     slopes, ws.status)
     workspace.publish_status(ws, "kv4_attn")
     return out, lse
 
@@ -184,8 +185,14 @@ def kv4_attn(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, lens: 
     return _attn(q, cache, block_table, lens, softmax_scale, softcap, alibi_slopes, False)[0]
 
 
-def kv4_attn_with_lse(q, cache, block_table, lens, softmax_scale=None, *, softcap=0.0,
-                      alibi_slopes=None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """As :func:`kv4_attn`, also returning the log-sum-exp ``[B, H_q, T]`` (fp32): what joins results over parts of a cache
-    that lies on several GPUs."""
-    return _attn(q, cache, block_table, lens, softmax_scale, softcap, alibi_slopes, True)
+def kv4_attn_with_lse(q, cache, block_table, lens, softmax_scale=None, *, softcap=0.0, alibi_slopes=None,
+                      tokens_after: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """As :func:`kv4_attn`, also returning the log-sum-exp ``[B, H_q, T]`` (fp32, -inf where a row sees no token).
+
+    Where the tokens of a sequence lie in several caches (on several GPUs, say), each in a part of its own, ``tokens_after``
+    (int32 ``[B]``) says how many of them lie behind the part in this one: query t is then token
+    ``lens[b] + tokens_after[b] - T + t`` of this part, and sees as much of it, at the distances, as it does of the whole.  With
+    ``w = exp(lse_part - logsumexp of all lse_part)`` the sum of ``w * out_part`` is the attention over the whole sequence
+    (``w = 0`` where a part's lse is -inf).
+    """
+    return _attn(q, cache, block_table, lens, softmax_scale, softcap, alibi_slopes, True, tokens_after)
