@@ -15,7 +15,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native, workspace
-from .scored import _check_slopes, _check_softcap
+from .scored import _check_slopes, _check_softcap, _refuse_tangents
 
 PAGE = 64    # tokens of a page
 GROUP = 32   # channels that share a scale and a minimum
@@ -101,7 +101,7 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, block_table: t
       positions: int32 ``[B]``: position of each sequence's first new token; token t goes to ``positions[b] + t``.
       counts: int32 ``[B]``: how many of the T tokens count (all of them by default).
     Tokens beyond the table, or on a page that is not in the pool, are left out; no other token of the cache changes.  The
-    result is unspecified where two tokens of one call go to the same place.
+    result is unspecified where two tokens of one call go to the same place.  The cache holds numbers: no gradient flows through it.
     """
     _check_tokens(k, cache, cache.n_kv_heads, "k")
     _check_tokens(v, cache, cache.n_kv_heads, "v")
@@ -151,6 +151,7 @@ def _attn(q, cache, block_table, lens, softmax_scale, softcap, alibi_slopes, wan
     slopes = _check_slopes(alibi_slopes, B, Hq, cache.device)
     if torch.is_grad_enabled() and q.requires_grad:
         raise RuntimeError("kv4_attn has no gradient: call it under torch.no_grad()")
+    _refuse_tangents("kv4_attn", q, alibi_slopes)
     _check_cuda(cache)
     if B == 0 or T == 0 or table.shape[1] == 0:
         out = torch.zeros((B, T, Hq, D), dtype=q.dtype, device=q.device)

@@ -18,6 +18,7 @@ import math
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native, schedule, workspace
@@ -232,6 +233,12 @@ class _ScoredFlashAttnFunc(torch.autograd.Function):
         return dq, dk, dv, None, None
 
 
+def _refuse_tangents(what: str, *tensors) -> None:
+    """Forward-mode differentiation: an output without a tangent would read as one of zero."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative")
+
+
 def _check_slopes(slopes: Optional[torch.Tensor], B: int, Hq: int, device: torch.device) -> Optional[torch.Tensor]:
     if slopes is None:
         return None
@@ -263,6 +270,7 @@ def _apply(q, k, v, softmax_scale, causal, softcap, alibi_slopes, mask, group) -
         raise ValueError("softmax_scale must be finite")
     if k.device != q.device or v.device != q.device:
         raise ValueError(f"q, k, v are on different devices: {q.device}, {k.device}, {v.device}")
+    _refuse_tangents("scored_flash_attn", q, k, v, alibi_slopes)
     B, S, Hq, _ = q.shape
     softcap = _check_softcap(softcap)
     slopes = _check_slopes(alibi_slopes, B, Hq, q.device)
