@@ -43,11 +43,13 @@ class DocumentMask:
         return self.buffer.device
 
     def update_(self, cu_seqlens, prefix_lens=None) -> "DocumentMask":
-        """Overwrites the mask in stream order with that of other documents (a replayed graph then sees them).  Calls whose
-        backward is still to come must not need the old one."""
+        """Overwrites the mask in stream order with that of other documents (a replayed graph then sees them).  A backward pass
+        that is still to come and needs the old one raises, as after any change in place of what autograd saved."""
         if (prefix_lens is not None) != self.has_prefix:
             raise ValueError("update_ takes prefix_lens exactly where the mask was made with them")
         cu, prefix = _borders(cu_seqlens, prefix_lens, self.batch, self.seq_len, self.device)
+        if not self.buffer.is_inference():
+            torch.autograd.graph.increment_version(self.buffer)
         _native.document_mask(cu, prefix, self.batch, self.seq_len // self.shards, self.shards, self.causal, self.buffer)
         return self
 
@@ -218,7 +220,10 @@ class _ScoredFlashAttnFunc(torch.autograd.Function):
         out, lse = _call(q, k, v, sc, group)
         ctx.sc, ctx.group = sc, group
         ctx.deterministic = _deterministic_now()
-        ctx.save_for_backward(q, k, v, out, lse)
+        # The scores read the slopes and the mask through their own references; saved as well, a change in place between the
+        # passes is found by their versions (which tensors made in inference mode do not have).
+        ctx.save_for_backward(q, k, v, out, lse, *(t if t is not None and not t.is_inference() else None
+                                                   for t in (sc.slopes, sc.mask)))
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return out, lse
@@ -226,7 +231,7 @@ class _ScoredFlashAttnFunc(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, _dlse=None):
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, lse, _, _ = ctx.saved_tensors
         if dout is None or q.numel() == 0:
             return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), None, None
         dq, dk, dv = _backward(ctx.group, _operand(dout), q, k, v, out, lse, ctx.sc.again(), ctx.deterministic)
@@ -304,7 +309,8 @@ def scored_flash_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax
     Args:
       q, k, v, softmax_scale, causal, group: as in :func:`ring_flash_attn`.
       softcap: scores are capped to ``softcap * tanh(score / softcap)``, softcap up to 1000; 0 leaves them as they are.
-      alibi_slopes: fp32 ``[H_q]`` or ``[B, H_q]``; ``slope * |i - j|`` is taken off the (capped) score.  Not differentiable.
+      alibi_slopes: fp32 ``[H_q]`` or ``[B, H_q]``; ``slope * |i - j|`` is taken off the (capped) score.  Not differentiable.  Slopes and mask must
+          stay as they are until the backward pass.
       mask: documents and prefixes, from :func:`document_mask` with the same ``causal`` and ``group``.
 
     Returns: out [B, S_local, H_q, D] in q's dtype; rows that see no key are zero.  Outside its padding (see
