@@ -63,6 +63,8 @@ def _int32(x: _Ints, device: torch.device, what: str) -> torch.Tensor:
         raise ValueError(f"{what} must be int32 or int64, got {t.dtype}")
     if t.is_cuda and t.device != device:
         raise ValueError(f"{what} is on {t.device}, the mask on {device}")
+    if t.dtype == torch.int64:  # what int32 cannot hold lies outside every sequence, on the same side as its ends
+        t = t.clamp(-1, 2 ** 31 - 1)
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 
