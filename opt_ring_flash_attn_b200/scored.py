@@ -108,6 +108,8 @@ def document_mask(cu_seqlens: _Ints, seq_len: int, *, prefix_lens: Optional[_Int
         device = cu_seqlens.device if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.is_cuda else torch.device(
             "cuda", torch.cuda.current_device()) if torch.cuda.is_available() else torch.device("cpu")
     device = torch.device(device)
+    if device.type == "cuda" and device.index is None:  # tensors say which one they are on
+        device = torch.device("cuda", torch.cuda.current_device())
     shards, _ = schedule._world(group)
     if seq_len < 1 or seq_len % shards != 0:
         raise ValueError(f"seq_len {seq_len} must be positive and a multiple of the {shards} ranks")

@@ -21,3 +21,20 @@ def test_masks_of_large_numbers():
                             prefix_lens=torch.tensor([2 ** 32 + 3, -2 ** 40], device=dev))
     assert torch.equal(got.buffer, want.buffer)
     assert torch.equal(rfa.document_mask([0, 100, 300], S, prefix_lens=[2 ** 40, 0], device=dev).buffer, want.buffer)
+
+
+def test_device_without_a_number(monkeypatch):
+    """``device="cuda"`` is the current device, also for borders that lie there already."""
+    seen = []
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    monkeypatch.setattr(scored, "_borders", lambda cu, pre, b, s, device: seen.append(device) or (cu, pre))
+    monkeypatch.setattr(scored._native, "mask_elems", lambda *a: (_ for _ in ()).throw(StopIteration))
+    with pytest.raises(StopIteration):
+        rfa.document_mask(torch.tensor([0, 16]), 16, device="cuda")
+    assert seen == [torch.device("cuda", 3)]
+
+
+@pytest.mark.gpu
+def test_borders_on_the_current_device():
+    mask = rfa.document_mask(torch.tensor([0, 100, 300], device="cuda"), 300, device="cuda")
+    assert mask.device == torch.device("cuda", torch.cuda.current_device())
