@@ -123,9 +123,13 @@ def document_mask(cu_seqlens: _Ints, seq_len: int, *, prefix_lens: Optional[_Int
         raise RuntimeError("document_mask runs on CUDA only (sm_100a kernels; there is no CPU path)")
     buffer = torch.empty(_native.mask_elems(batch, seq_len // shards, shards), dtype=torch.int32, device=device)
     _native.document_mask(cu, prefix, batch, seq_len // shards, shards, causal, buffer)
-    # with n documents a long one holds some twice the mean; their borders stay on the device
     return DocumentMask(buffer, batch, seq_len, shards, bool(causal), prefix is not None,
-                        min(seq_len, 2 * seq_len // (cu.shape[-1] - 1)))
+                        _typical_keys(seq_len, cu.shape[-1] - 1))
+
+
+def _typical_keys(seq_len: int, documents: int) -> int:
+    """What a long one of them holds, some twice the mean; their borders stay on the device.  Never 0, which would say: all."""
+    return max(1, min(seq_len, 2 * seq_len // documents))
 
 
 class _Scores:

@@ -38,3 +38,9 @@ def test_device_without_a_number(monkeypatch):
 def test_borders_on_the_current_device():
     mask = rfa.document_mask(torch.tensor([0, 100, 300], device="cuda"), 300, device="cuda")
     assert mask.device == torch.device("cuda", torch.cuda.current_device())
+
+
+def test_typical_keys_of_many_documents():
+    """More borders than tokens (rows padded to a fixed number of documents): short documents, not one long one."""
+    assert scored._typical_keys(1000, 1) == 1000 and scored._typical_keys(1000, 10) == 200
+    assert scored._typical_keys(1000, 5000) == 1
