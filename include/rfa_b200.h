@@ -238,7 +238,7 @@ int rfa_bwd_local(const void* q, const void* k, const void* v, const void* out, 
  * mask buffer names.  A row that sees no key gets out = 0 and lse = -inf, and takes no part in any gradient.
  */
 typedef struct rfa_score_args {
-  float softmax_scale;      /* > 0 */
+  float softmax_scale;      /* > 0; 1.45 times it, and 2.9 times over softcap, must stay in fp32 */
   float softcap;            /* up to 1000: cap of the scores; 0: none */
   const float* slopes;      /* NULL, or distance slopes (>= 0 or < 0): [Hq], or [B, Hq] with slopes_per_batch */
   int slopes_per_batch;

@@ -1225,7 +1225,7 @@ extern "C" int rfa_kv4_attn_part(const void* q, const long long* q_strides, cons
   const int rc = kv4_check(codes, meta, n_pages, table, max_pages, lens, B, T, Hkv, D, dtype);
   if (rc != RFA_OK) return rc;
   if (Hq <= 0 || Hq % Hkv != 0) return RFA_ERR_INVALID_ARG;
-  if (!(softmax_scale > 0.f) || !(softmax_scale <= 3.0e38f) || !(softcap >= 0.f) || !(softcap <= kMaxCap))
+  if (!(softmax_scale > 0.f) || !(softcap >= 0.f) || !scores_fit(softmax_scale, softcap))
     return RFA_ERR_INVALID_ARG;
   for (int i = 0; i < 3; ++i)
     if (q_strides[i] % 8 != 0) return RFA_ERR_INVALID_ARG;

@@ -75,10 +75,15 @@ struct ScoreParams {
   MaskView mask;
 };
 
+// What the kernels multiply raw scores with has to be a number: scale * log2(e) and, for the tanh, 2 * scale * log2(e) / cap.
+inline bool scores_fit(float scale, float cap) {
+  return cap <= kMaxCap && 1.45 * scale <= 3.4e38 && (!(cap > 0.f) || 2.9 * scale <= 3.4e38 * cap);
+}
+
 // Checks and unpacks the arguments of an entry point.
 inline int make_score_params(const rfa_score_args* a, int B, int S, ScoreParams* out) {
   if (!a || !(a->softmax_scale > 0.f) || !(a->softcap >= 0.f)) return RFA_ERR_INVALID_ARG;
-  if (!(a->softmax_scale <= 3.0e38f) || !(a->softcap <= kMaxCap)) return RFA_ERR_INVALID_ARG;
+  if (!scores_fit(a->softmax_scale, a->softcap)) return RFA_ERR_INVALID_ARG;
   if (a->shards < 1 || a->q_shard < 0 || a->q_shard >= a->shards || a->k_shard < 0 || a->k_shard >= a->shards)
     return RFA_ERR_INVALID_ARG;
   if (static_cast<long long>(S) * a->shards > INT_MAX / 2) return RFA_ERR_TOO_LARGE;

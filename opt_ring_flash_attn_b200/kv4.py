@@ -147,7 +147,7 @@ def _attn(q, cache, block_table, lens, softmax_scale, softcap, alibi_slopes, wan
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not (scale > 0) or math.isinf(scale):
         raise ValueError("softmax_scale must be positive and finite")
-    softcap = _check_softcap(softcap)
+    softcap = _check_softcap(softcap, scale)
     slopes = _check_slopes(alibi_slopes, B, Hq, cache.device)
     if torch.is_grad_enabled() and q.requires_grad:
         raise RuntimeError("kv4_attn has no gradient: call it under torch.no_grad()")

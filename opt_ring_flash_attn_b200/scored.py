@@ -268,10 +268,15 @@ def _check_slopes(slopes: Optional[torch.Tensor], B: int, Hq: int, device: torch
     return slopes.contiguous()
 
 
-def _check_softcap(softcap: float) -> float:
+def _check_softcap(softcap: float, softmax_scale: float) -> float:
     softcap = float(softcap or 0.0)
     if not (0.0 <= softcap <= MAX_SOFTCAP):
         raise ValueError(f"softcap must be 0 (none) or a positive number up to {MAX_SOFTCAP:g}, got {softcap}")
+    # the kernels work with scale * log2(e) and, for the tanh, 2 * scale * log2(e) / softcap in fp32
+    if not (softmax_scale * 1.45 <= 3.4e38):
+        raise ValueError(f"softmax_scale {softmax_scale:g} is too large for fp32")
+    if softcap > 0 and not (softmax_scale * 2.9 <= 3.4e38 * softcap):
+        raise ValueError(f"softcap {softcap:g} is too small for softmax_scale {softmax_scale:g}")
     return softcap
 
 
@@ -287,7 +292,7 @@ def _apply(q, k, v, softmax_scale, causal, softcap, alibi_slopes, mask, group) -
         raise ValueError(f"q, k, v are on different devices: {q.device}, {k.device}, {v.device}")
     _refuse_tangents("scored_flash_attn", q, k, v, alibi_slopes)
     B, S, Hq, _ = q.shape
-    softcap = _check_softcap(softcap)
+    softcap = _check_softcap(softcap, softmax_scale)
     slopes = _check_slopes(alibi_slopes, B, Hq, q.device)
     causal = bool(causal)
     world, rank = schedule._world(group)
