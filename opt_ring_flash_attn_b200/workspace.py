@@ -20,6 +20,7 @@ the word has to reach the host: :func:`publish_status` copies it out asynchronou
 from __future__ import annotations
 
 import os
+import threading
 import time
 from dataclasses import dataclass, field
 from typing import Any, Dict, List, Optional, Tuple
@@ -104,6 +105,7 @@ def _retire(ws) -> None:
 # device -> status word of the operators that allocate their scratch per call (any number of streams may use it: a kernel
 # writes it only where it fails)
 _status_cache: Dict[torch.device, ForwardWorkspace] = {}
+_status_lock = threading.Lock()
 
 
 def all_workspaces() -> List:
@@ -114,16 +116,23 @@ def status_workspace(device: torch.device) -> ForwardWorkspace:
     """The status word of a device, with its pinned copy.  The first use must not be inside a graph capture."""
     ws = _status_cache.get(device)
     if ws is None:
-        if device.type == "cuda":
-            with torch.cuda.device(device):
-                if torch.cuda.is_current_stream_capturing():
-                    raise RuntimeError("the first call on a device sets up its status word: make one before capturing a graph")
-                status, host = _new_status(device)
-                torch.cuda.current_stream(device).synchronize()  # other streams may read the word from now on
-        else:
-            status, host = _new_status(device)
-        ws = _status_cache[device] = ForwardWorkspace(None, None, None, None, [], status, host)
+        with _status_lock:  # two threads' first calls get the same word: kernels of either go on reading it
+            ws = _status_cache.get(device)
+            if ws is None:
+                ws = _status_cache[device] = _new_status_workspace(device)
     return ws
+
+
+def _new_status_workspace(device: torch.device) -> ForwardWorkspace:
+    if device.type == "cuda":
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first call on a device sets up its status word: make one before capturing a graph")
+            status, host = _new_status(device)
+            torch.cuda.current_stream(device).synchronize()  # other streams may read the word from now on
+    else:
+        status, host = _new_status(device)
+    return ForwardWorkspace(None, None, None, None, [], status, host)
 
 
 def _fail(ws, code: int, what: str):
