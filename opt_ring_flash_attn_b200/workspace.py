@@ -250,8 +250,9 @@ def backward_workspace(q: torch.Tensor, k: torch.Tensor, world_size: int,
 
 
 def clear() -> None:
+    """Drops the scratch of the ring schedules.  The status words stay (4 bytes per device): captured graphs of the operators
+    that have no other scratch of ours may still be replayed, and their kernels read them."""
     for ws in all_workspaces():
         _retire(ws)
     _fwd_cache.clear()
     _bwd_cache.clear()
-    _status_cache.clear()

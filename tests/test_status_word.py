@@ -23,3 +23,10 @@ def test_first_calls_of_two_threads_share_the_word(monkeypatch):
     for t in threads:
         t.join()
     assert len(got) == 4 and all(ws is got[0] for ws in got)
+
+
+def test_the_word_outlives_the_scratch():
+    """A captured decoding step is replayed after ``shutdown()``: its kernels read the word they were captured with."""
+    ws = workspace.status_workspace(torch.device("cpu"))
+    workspace.clear()
+    assert workspace.status_workspace(torch.device("cpu")) is ws
