@@ -399,22 +399,6 @@ struct Kv4Fetch {
   }
 };
 
-// The two halves of a meta word in fp32, by additions of mixed precision: a shift or a mask would go to the logic unit.
-template <typename T>
-__device__ __forceinline__ float wide_lo(uint32_t w) {
-  float y;
-  if constexpr (Pack2<T>::kIsBf16) asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tadd.rn.f32.bf16 %0, l, %2;\n\t}" : "=f"(y) : "r"(w), "f"(-0.f));
-  else asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tadd.rn.f32.f16 %0, l, %2;\n\t}" : "=f"(y) : "r"(w), "f"(-0.f));
-  return y;
-}
-template <typename T>
-__device__ __forceinline__ float wide_hi(uint32_t w) {
-  float y;
-  if constexpr (Pack2<T>::kIsBf16) asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tadd.rn.f32.bf16 %0, h, %2;\n\t}" : "=f"(y) : "r"(w), "f"(-0.f));
-  else asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tadd.rn.f32.f16 %0, h, %2;\n\t}" : "=f"(y) : "r"(w), "f"(-0.f));
-  return y;
-}
-
 // Codes e and e + 4 of a word (one per half word) as fp16, (u - 8) or u times 2^-24 (e even) or 2^-20 (e odd).
 template <bool kCentred, int e>
 __device__ __forceinline__ uint32_t codes_fp16(uint32_t w) {
