@@ -1,8 +1,8 @@
 """Serving what the operators of this package train: a paged K/V cache held in 4 bits, and the attention of new tokens over it.
 
 ``kv4_append`` puts tokens into the cache, ``kv4_attn`` lets the last tokens of every sequence attend to all of it (with the
-capped and distance-biased scores of :func:`scored_flash_attn`), ``kv4_gather`` reads tokens back, for the next part of a
-prompt or to look at them.  Each call is asynchronous on the current stream; positions and lengths are read on the device, so
+capped and distance-biased scores of :func:`scored_flash_attn`): one token, a few drafted ones, or the next part of a prompt.
+``kv4_gather`` reads tokens back.  Each call is asynchronous on the current stream; positions and lengths are read on the device, so
 a decoding step can be captured into a CUDA graph and replayed as the sequences grow.
 
 The reference has no serving path; the scores follow its ``alibi_slopes`` arguments (ring_flash_attn.py:385-463).
@@ -174,7 +174,8 @@ def kv4_attn(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, lens: 
     """Attention of the last T tokens of every sequence over its tokens in the cache (their own included: append first).
 
     Args:
-      q: ``[B, T, H_q, D]`` in the cache's dtype: one token (T = 1) or a few, e.g. drafted ones.
+      q: ``[B, T, H_q, D]`` in the cache's dtype: one token (T = 1), a few drafted ones, or the next part of a prompt.  The
+          cache is read once for every 16 rows (8 above head dim 128) of T times the group's heads.
       block_table: int32 ``[B, max_pages]`` as for :func:`kv4_append`.
       lens: int32 ``[B]``: tokens of each sequence in the cache; query t is token ``lens[b] - T + t`` and sees the tokens up to
           itself.  Lengths beyond the table end at it; tokens on a page that is not in the pool do not exist.

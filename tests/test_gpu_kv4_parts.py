@@ -89,3 +89,21 @@ def test_offsets_at_the_ends_of_int32():
     out, lse = rfa.kv4_attn_with_lse(q, *parts[0], _ints([100] * 4), tokens_after=_ints([-2 ** 31, -1, 0, 2 ** 31 - 1]))
     rfa.check("test")
     check(out, lse, reference(q, *parts[0], [100] * 4, after=[0, 0, 0, 2 ** 31 - 101]))
+
+
+@pytest.mark.parametrize("D,dt,Hq,Hkv,size", [(128, BF, 8, 2, 130), (64, HF, 4, 4, 64), (256, BF, 4, 1, 100), (96, HF, 6, 2, 257)])
+def test_a_prompt_in_parts(D, dt, Hq, Hkv, size):
+    """A prompt goes in part by part: each part is appended and attends to all that is cached, a ragged last one too."""
+    import opt_ring_flash_attn_b200 as rfa
+
+    B, S = 2, 600
+    x = [torch.randn(B, S, h, D, generator=_gen(45 + i), device=DEV).to(dt) for i, h in enumerate((Hq, Hkv, Hkv))]
+    slopes = torch.tensor([2.0 ** (-4.0 * (h + 1) / Hq) for h in range(Hq)], device=DEV)
+    table, n = _table([S] * B)
+    cache = rfa.KV4Cache.empty(n, Hkv, D, dt, DEV)
+    for a in range(0, S, size):
+        e = min(S, a + size)
+        rfa.kv4_append(cache, x[1][:, a:e], x[2][:, a:e], table, _ints([a] * B))
+        out, lse = rfa.kv4_attn_with_lse(x[0][:, a:e], cache, table, _ints([e] * B), softcap=20.0, alibi_slopes=slopes)
+        rfa.check("test")
+        check(out, lse, reference(x[0][:, a:e], cache, table, [e] * B, softcap=20.0, slopes=slopes))
