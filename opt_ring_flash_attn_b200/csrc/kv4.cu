@@ -493,7 +493,8 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
   __shared__ int page_ok[2][kRing];
   __shared__ Kv4Fetch fetcher[2];
   // per warp, in shared memory because registers are short: powers of two on the scales of V per group, slopes per column
-  __shared__ __align__(16) float v_down_s[4][NG], slope_s[4][8 * NT];
+  __shared__ __align__(16) uint32_t v_down_s[4][NG];  // (as bits)
+  __shared__ float slope_s[4][8 * NT];
   __shared__ int abort_flag, skip_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -634,7 +635,7 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
       }
     }
     float o[NT][NG][2][4], corr[NT][NG][2], m[NT][2], l[NT][2];
-    if (lane < NG) v_down_s[warp][lane] = kMostDown;
+    if (lane < NG) v_down_s[warp][lane] = __float_as_uint(kMostDown);
     __syncwarp();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -805,9 +806,11 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
             }
           }
           float sc0[NG], sc1[NG], most = 0.f, v_down[NG];
-          lds_words<NG>(reinterpret_cast<uint32_t(&)[NG]>(v_down), reinterpret_cast<const uint8_t*>(v_down_s[warp]));
+          uint32_t down_bits[NG];
+          lds_words<NG>(down_bits, reinterpret_cast<const uint8_t*>(v_down_s[warp]));
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
+            v_down[g] = __uint_as_float(down_bits[g]);
             sc0[g] = Kv4Type<T>::lo(e0[g]) * v_down[g];
             sc1[g] = Kv4Type<T>::lo(e1[g]) * v_down[g];
             most = fmaxf(fmaxf(most, fabsf(sc0[g])), fabsf(sc1[g]));
@@ -823,7 +826,7 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
               const float down = change ? __uint_as_float((258u - (top >> 23)) << 23) : v_down[g];
               const float f = down * power_rcp(v_down[g]);
               v_down[g] = down;
-              if (lane == 0) v_down_s[warp][g] = down;
+              if (lane == 0) v_down_s[warp][g] = __float_as_uint(down);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -923,7 +926,7 @@ __global__ void __launch_bounds__(128, Kv4Cfg<NG, NT>::kBlocksPerSm) kv4_attn_ke
             const float f = fast_exp2(m[nt][x] - top[nt][x]);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {  // channels 32 g + 4 r + (0..3); even codes carry 2^24, odd ones 2^20
-              const float up = f * power_rcp(v_down_s[warp][g]);
+              const float up = f * power_rcp(__uint_as_float(v_down_s[warp][g]));
               float4* dst = reinterpret_cast<float4*>(join + (pair * kRows + nt * 8 + 2 * c + x) * D + g * kGroup + 4 * r);
               const float4 old = w == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *dst;
               const float rest = corr[nt][g][x] * f;

@@ -25,7 +25,7 @@ HEAD_DIMS = (64, 96, 128, 192, 256)
 class KV4Cache:
     """A pool of pages of 64 tokens.  ``codes`` is uint8 ``[n_pages, H_kv, 2, 64, D / 2]`` (K, then V), ``meta`` bf16 or fp16
     ``[n_pages, H_kv, 2, 64, D / 32, 2]``: scale and minimum of every 32 channels; a code u stands for ``u * scale + minimum``
-    (2.5 to 3.2 times smaller than 16 bits).  The order of the codes inside a row is that of ``rfa_kv4_append`` in the C header.
+    (5 bits a value, 3.2 times smaller than 16).  The order of the codes inside a row is that of ``rfa_kv4_append`` in the C header.
     Both tensors belong to the caller: which page holds which tokens is said by the block table of each call."""
 
     def __init__(self, codes: torch.Tensor, meta: torch.Tensor):
@@ -182,7 +182,10 @@ def kv4_attn(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, lens: 
       softmax_scale, softcap, alibi_slopes: as in :func:`scored_flash_attn`.
 
     Returns: out ``[B, T, H_q, D]``; rows that see no token are zero.  What the pages hold behind the last token does not
-    matter; the tokens themselves must be finite (of T > 1, a row may take up a NaN of a token behind it).  Results do not depend on how the work is split: the same call gives the same bits.
+    matter; the tokens themselves must be finite (of T > 1, a row may take up a NaN of a token behind it), and like q so far from
+    the largest numbers that a sequence's sums stay in fp32.  The weights times the scales of V are rounded to 11 bits, relative to
+    the largest scale of their 32 channels; what lies 2^-18 or more below it keeps fewer.  The same call gives the same bits; the
+    other sequences of a batch decide how the work is split, so another batch may give the last bits differently.
     """
     return _attn(q, cache, block_table, lens, softmax_scale, softcap, alibi_slopes, False)[0]
 
