@@ -242,12 +242,12 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(T* __restrict__ k, T* _
 // head, tile of query rows) laid end to end, block i takes pages [i q, (i + 1) q) of them all, whatever the lengths are.  A
 // unit that several blocks share is joined by a second kernel from at most two partial results per block.
 //
-// Measured (pages scattered, lengths to 8192 / two of 131072; 32/8 heads of 128): 92 and 79 us for 335 and 286 MB, 3.7 TB/s; the
+// Measured (pages scattered, lengths to 8192 / two of 131072; 32/8 heads of 128): 93 and 81 us for 335 and 286 MB, 3.6 TB/s; the
 // longer the cache the nearer to 4.7 TB/s (8 x as long), the copies alone take 72 and 62.  The logic unit is 52 % busy, issue
 // 55 %; some 15 us are the start, the joining of warps and the second launch.  One sequence of 1000: 12 us.  Steps on the way:
 // a fifth warp for the copies 144 / 118 us (it costs registers: five warps on four schedulers); products in e4m3 161 / 126; fp16
 // subnormals 141 / 104; parts of a unit read with loads in flight instead of in turn 104 -> 89; a cost per unit in the sharing
-// out 139 -> 97; columns folded 97 / 84 -> 92 / 79.  More work for the warps that an SM favours (the older ones) changes nothing.
+// out 139 -> 97; columns folded 97 / 84 -> 92 / 79; powers of V's scales per group 92 / 80 -> 93 / 81.  More work for the warps that an SM favours (the older ones) changes nothing.
 //
 // A block has two pairs of warps; a pair takes every other page of a run, a warp 32 of its 64 tokens, and the pair's first
 // warp keeps its pages coming through a ring of its own.  Tokens are the 16 rows, query rows (tokens x heads of the group, 8
@@ -263,8 +263,8 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(T* __restrict__ k, T* _
 //   P sc is rounded to fp16 (11 bits, for bf16 caches too), under a power of two per group of 32 channels that brings the
 //   largest scale of V that the run has met to 2^4 or more (weights are 4 at most).  So P sc loses bits where it is less than 2^-18 of the
 //   group's largest scale, at most 2^-29 of that scale a token.  (One power for all groups took the bits from the small ones: beside
-//   a group 2^17 times as large, results were off by 7 %.)  The powers lie in shared memory: in registers, which the kernel has none
-//   to spare of, b64 below takes 97 us, with one power for all 92.
+//   a group 2^17 times as large, results were off by 7 %.)  The powers lie in shared memory: in registers, of which the kernel has none
+//   to spare, the first case above takes 97 us.
 //   For fp16 results u - 8 stands in for u, which halves what that rounding weighs (min + 8 sc makes up for it): relative error of fp16
 //   results 2.8e-4 instead of 4.8e-4, where rounding the result alone gives 2.1e-4.
 constexpr float kMostDown = 2.6584559915698317e36f;  // 2^121, what scales of V are multiplied with before any was seen

@@ -14,7 +14,8 @@
 namespace rfa {
 
 constexpr float kLog2e = 1.4426950408889634f;
-// Largest cap: cap * tanh comes out of cap - 2 cap / (exp + 1) with an error of 2^-24 cap, 6e-5 of a weight here.
+// Largest cap: cap * tanh comes out of cap - 2 cap / (exp + 1) with an error of up to 9 * 2^-24 of the cap (exp2 2^-22, reciprocal
+// 2^-23, three roundings), or of a polynomial with 3.5e-7 (scored_fwd.cu): 5e-4 of a weight here, about what its rounding to fp16 is.
 constexpr float kMaxCap = 1000.f;
 // Running maximum of a row that has seen no key: finite, so that exp2(-inf - kNoKey) is 0 and not NaN, and far below any
 // score in log2 units that could matter, so that the first real one rescales what was there by 0.

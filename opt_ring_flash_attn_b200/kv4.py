@@ -102,6 +102,7 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, block_table: t
       counts: int32 ``[B]``: how many of the T tokens count (all of them by default).
     Tokens beyond the table, or on a page that is not in the pool, are left out; no other token of the cache changes.  The
     result is unspecified where two tokens of one call go to the same place.  The cache holds numbers: no gradient flows through it.
+    A group with a NaN, an infinity, or values further apart than fp32's largest number reads back as no numbers.
     """
     _check_tokens(k, cache, cache.n_kv_heads, "k")
     _check_tokens(v, cache, cache.n_kv_heads, "v")

@@ -25,7 +25,7 @@ from . import _native, schedule, workspace
 from .api import _deterministic_now, _validate
 
 
-MAX_SOFTCAP = 1000.0  # above, the tanh would lose too much in fp32
+MAX_SOFTCAP = 1000.0  # here the tanh is off by 5e-4 of a score (fp32)
 
 
 class DocumentMask:
@@ -327,7 +327,8 @@ def scored_flash_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax
       mask: documents and prefixes, from :func:`document_mask` with the same ``causal`` and ``group``.
 
     Returns: out [B, S_local, H_q, D] in q's dtype; rows that see no key are zero.  Outside its padding (see
-    :func:`document_mask`) K and V must be finite: an infinity or a NaN reaches rows that do not see it.
+    :func:`document_mask`) K and V must be finite: an infinity or a NaN reaches rows that do not see it.  (In bf16 without a cap a
+    masked key may keep a weight of 2^-125 of the row's largest: V has to stay below 1e30 there.)
     :func:`deterministic` holds here too, at the price of visiting every tile of a masked block.
     """
     return _apply(q, k, v, softmax_scale, causal, softcap, alibi_slopes, mask, group)[0]
