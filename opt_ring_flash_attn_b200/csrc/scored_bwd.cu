@@ -8,7 +8,7 @@
 // fp32 accumulator.  What differs:
 //  * The key rows of a CTA have intervals of queries that see them; their hull gives the query tiles it walks, and a thread
 //    (= key row) compares a query with its own interval in the tiles that are not inside all of them.
-//  * What the second half of a tile's work needs of the scores is one factor, W = P (1 - tanh^2), kept as 16-bit pairs in the
+//  * What the second half of a tile's work needs of the scores is one factor, W = P (1 - tanh^2), kept as pairs of fp16 in the
 //    registers that hold P in the plain hop; P itself goes to tensor memory at once.
 //  * The issuing warp clears the padding rows of K, Q and dO tiles on the border between real rows and padding.
 //  * A key tile that no query sees writes zeros.
@@ -19,9 +19,10 @@
 // 570.  (A cap with a running bias of 0 instead of an instantiation of its own: 499, 230, 578.)
 // Taking the tile coordinates out of registers (BwdPlan) was worth 12 to 20 %: 199 -> 159 us (16 heads of 64 with a bias).  A
 // polynomial for the tanh, as in the forward hop, loses here: 517 -> 556 us; the special-function unit is not what binds.
-// dQ and dK carry three roundings to 16 bits: W (there are registers for P's pairs, not for fp32), dX (an operand of the products) and
-// the result, and delta that of out: relative error 3.0e-3 to 3.7e-3 in bf16, 5e-4 in fp16, where the result's rounding alone
-// gives 1.7e-3 and 2.1e-4.
+// dQ and dK carry roundings to 16 bits of W (there are registers for pairs, not for fp32; fp16 whatever the operands are, see
+// weight_shift), of dX (an operand of the products) and of the result, and delta that of out: relative error 2.5e-3 to 3.0e-3 in
+// bf16 (3.0e-3 to 3.6e-3 with W in bf16, no faster but for plain scores at head dim 128: 386 for 392 us), 4e-4 to 5e-4 in fp16; the
+// result's rounding alone gives 1.7e-3 and 2.1e-4.
 #include <initializer_list>
 #include <type_traits>
 
@@ -29,6 +30,11 @@
 #include "scored.cuh"
 
 namespace rfa {
+
+// With bf16 operands P and dX are 2^15 times themselves (the results are scaled back), which lets W, whose type no product
+// sees, be fp16: 11 bits instead of 8 down to weights of 2^-29, less below.
+template <typename T>
+__host__ __device__ constexpr int weight_shift() { return Pack2<T>::kIsBf16 ? 15 : 0; }
 
 struct ScoredBwdParams {
   BwdParams p;
@@ -191,6 +197,7 @@ __global__ void __launch_bounds__(640, 1)
   const ScoreParams& sc = prm.sc;
   using Cfg = ScoredBwdCfg<DP, DH, BQ, NSQ, NSO>;
   constexpr bool kBf16 = Pack2<T>::kIsBf16;
+  constexpr int kShift = weight_shift<T>();
   constexpr int kPanelK = 128 * 128;  // bytes per panel of a 128-row tile
   constexpr int kPanelQ = BQ * 128;   // bytes per panel of a BQ-row tile
 
@@ -553,7 +560,7 @@ __global__ void __launch_bounds__(640, 1)
       tc_fence_after_sync();
       const int q0 = i * BQ + col0;
       const bool masked = i * BQ < full_lo || i * BQ + BQ > full_hi;
-      uint32_t pk[NCH * 16];  // W = P (1 - tanh^2) for dX, in 16 bits like the P of the dV product
+      uint32_t pk[NCH * 16];  // W = P (1 - tanh^2) for dX, in fp16
       {
         uint32_t r[NCH][32];
 #pragma unroll
@@ -576,16 +583,16 @@ __global__ void __launch_bounds__(640, 1)
             uint32_t u[16];
             const int d = ahead + i * BQ + c * 32;
             uint64_t bias = 0;
-            if (kKind > 0) {
-              // what y has beside lse2: the distance and the constant of the tanh
-              const float b0 = (has_bias(kKind) && kLinear ? static_cast<float>(d) * sign_slope : 0.f) - (has_cap(kKind) ? cap_log2 : 0.f);
+            if (kKind > 0 || kShift > 0) {
+              // what y has beside lse2: the distance, the constant of the tanh, the power of two on P
+              const float b0 = (has_bias(kKind) && kLinear ? static_cast<float>(d) * sign_slope : 0.f) - (has_cap(kKind) ? cap_log2 + kShift : kShift);
               bias = pack_f2(b0, has_bias(kKind) && kLinear ? b0 + sign_slope : b0);
             }
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               const float2 l2 = *reinterpret_cast<const float2*>(lse2_s + c * 32 + k * 2);
               uint64_t y2 = pack_f2(l2.x, l2.y);
-              if (kKind > 0) {
+              if (kKind > 0 || kShift > 0) {
                 y2 = add2(y2, bias);
                 if (has_bias(kKind) && kLinear) bias = add2(bias, step);
                 else if (has_bias(kKind)) y2 = add2(y2, pack_f2(slope * fabsf(static_cast<float>(d + 2 * k)), slope * fabsf(static_cast<float>(d + 2 * k + 1))));
@@ -615,9 +622,9 @@ __global__ void __launch_bounds__(640, 1)
               if constexpr (has_cap(kKind)) {
                 float w0, w1;
                 unpack_f2(mul2(pack_f2(e0, e1), jac2), w0, w1);
-                pk[c * 16 + k] = Pack2<T>::pack(w0, w1);
+                pk[c * 16 + k] = Pack2<__half>::pack(w0, w1);
               } else {
-                pk[c * 16 + k] = u[k];
+                pk[c * 16 + k] = kBf16 ? Pack2<__half>::pack(e0, e1) : u[k];
               }
             }
             // P^T (16 bit, two per column) goes over the start of this group's own S^T columns, all of which are in registers
@@ -653,8 +660,8 @@ __global__ void __launch_bounds__(640, 1)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const float4 d4 = *reinterpret_cast<const float4*>(delta_s + c * 32 + k * 4);
-            const float2 p01 = Pack2<T>::unpack(pk[c * 16 + 2 * k + 0]);
-            const float2 p23 = Pack2<T>::unpack(pk[c * 16 + 2 * k + 1]);
+            const float2 p01 = Pack2<__half>::unpack(pk[c * 16 + 2 * k + 0]);
+            const float2 p23 = Pack2<__half>::unpack(pk[c * 16 + 2 * k + 1]);
             float s0, s1, s2, s3;
             unpack_f2(mul2(pack_f2(p01.x, p01.y),
                            sub2(pack_u2(r[c][4 * k + 0], r[c][4 * k + 1]), pack_f2(d4.x, d4.y))), s0, s1);
@@ -693,7 +700,7 @@ __global__ void __launch_bounds__(640, 1)
       tc_fence_after_sync();
       const bool row_ok = kvpos < p.Skv;
       const int which = (cw == 0) ? 1 : 0;  // packed buffer: [0] = dK, [1] = dV
-      const float mul = (cw == 0) ? 1.0f : p.scale;
+      const float mul = (cw == 0) ? 1.0f / (1 << kShift) : p.scale;
       const uint32_t a_acc = tmem_base + lane_addr + (cw == 0 ? Cfg::kTmDV : Cfg::kTmDK);
       T* const out16 = static_cast<T*>(cw == 0 ? p.dv16 : p.dk16);
       const size_t base16 = ((static_cast<size_t>(b) * p.Skv + kvpos) * p.Hkv + hkv) * p.D + hf * DH;
@@ -927,7 +934,7 @@ static int scored_dispatch(const void* q, const void* k, const void* v, const vo
 }
 
 static int scored_bwd_params(const void* k, const float* lse2, const float* delta, float* dq_acc, float* dkdv_out, int B,
-                             int S, int Hq, int Hkv, int D, const rfa_score_args* args, int* dq_order, int* status,
+                             int S, int Hq, int Hkv, int D, int dtype, const rfa_score_args* args, int* dq_order, int* status,
                              ScoredBwdParams* prm) {
   const int rc = make_score_params(args, B, S, &prm->sc);
   if (rc != RFA_OK) return rc;
@@ -944,7 +951,8 @@ static int scored_bwd_params(const void* k, const float* lse2, const float* delt
   p.Hkv = Hkv;
   p.D = D;
   p.Spad = round_up(S, 128);
-  p.scale = args->softmax_scale;
+  // of dQ and dK
+  p.scale = args->softmax_scale / (1 << (dtype == RFA_DTYPE_BF16 ? weight_shift<__nv_bfloat16>() : weight_shift<__half>()));
   p.scale_log2 = args->softmax_scale * kLog2e;
   // the shape of the work that the split of the K/V tiles is chosen for: documents only shorten it
   p.causal = prm->sc.causal && prm->sc.q_pos == prm->sc.k_pos ? 1 : 0;
@@ -983,7 +991,7 @@ extern "C" int rfa_scored_bwd_hop(const void* q, const void* k, const void* v, c
   if (rc != RFA_OK) return rc;
   if (misaligned({dq_acc, k}) || (reinterpret_cast<uintptr_t>(dq_order) & 3u)) return RFA_ERR_INVALID_ARG;
   ScoredBwdParams prm;
-  rc = scored_bwd_params(k, lse2, delta, dq_acc, dkdv_out, B, S, Hq, Hkv, D, args, dq_order, status, &prm);
+  rc = scored_bwd_params(k, lse2, delta, dq_acc, dkdv_out, B, S, Hq, Hkv, D, dtype, args, dq_order, status, &prm);
   if (rc != RFA_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if ((rc = prepare_dkdv(prm.p, s)) != RFA_OK) return rc;
@@ -1003,7 +1011,7 @@ extern "C" int rfa_scored_bwd_local(const void* q, const void* k, const void* v,
   if (rc != RFA_OK) return rc;
   if (misaligned({dq_acc, dq, dk, dv, dq_order, out, dout, k})) return RFA_ERR_INVALID_ARG;
   ScoredBwdParams prm;
-  rc = scored_bwd_params(k, lse2, delta, dq_acc, dkdv, B, S, Hq, Hkv, D, args, dq_order, status, &prm);
+  rc = scored_bwd_params(k, lse2, delta, dq_acc, dkdv, B, S, Hq, Hkv, D, dtype, args, dq_order, status, &prm);
   if (rc != RFA_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   ClearList clear;
