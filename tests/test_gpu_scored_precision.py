@@ -45,3 +45,17 @@ def test_gradients(D, dt, cap):
     for name, e, c in zip(("dq", "dk"), exact, coarse):
         off, expected = (got[name].double() - e).norm() / e.norm(), (c - e).norm() / e.norm()
         assert off <= (1.05 if dt == BF else 1.15) * expected, f"{name}: {off.item():.2e}, the roundings alone {expected.item():.2e}"
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("kind", ["plain", "bias"])
+def test_scores_that_lse_cannot_hold(D, kind):
+    """Scores of 10^7 to 5 * 10^8: lse keeps no more than their leading digits, so weights come out too large; what flows back stays
+    finite.  (Below 2^29 in log2 units neighbouring numbers are 32 apart: maximum and lse are off by 16 each, a weight by 2^32, and
+    under 2^15 that is still far inside fp32 and bf16.  From 2^32 on they are 512 apart, and the forward pass itself, plain or not,
+    overflows in exp2: there is nothing to hold.)"""
+    q, k, v, dout = inputs(71, 1, 300, 2, 2, D, BF, DEV)
+    slopes = torch.full((2,), 0.1, device=DEV) if kind == "bias" else None
+    for std in (2.0 ** 12, 2.0 ** 13):
+        got = _run(q * std * (64 / D) ** 0.25, k * std * (64 / D) ** 0.25, v, dout, causal=True, alibi_slopes=slopes)
+        assert all(torch.isfinite(got[n]).all() for n in got)
