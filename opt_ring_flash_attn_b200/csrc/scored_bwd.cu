@@ -27,6 +27,7 @@
 #include <type_traits>
 
 #include "bwd_common.cuh"
+#include "bwd_tile.cuh"
 #include "scored.cuh"
 
 namespace rfa {
@@ -49,72 +50,6 @@ __device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
 struct ScoredBwdParams {
   BwdParams p;
   ScoreParams sc;
-};
-
-constexpr unsigned kRedSleepNs = 100;  // pause between the vector reductions of head dim 256, as in the plain hop
-
-namespace {
-
-// Bounded wait of one lane until a counter in global memory has reached `target`; the whole warp gets the answer
-// (false: the CTA is aborting).
-__device__ __forceinline__ bool wait_count(const int* sem, int target, bool waiter, volatile int* abort_p) {
-  bool got = true;
-  if (waiter) {
-    const unsigned long long since = global_timer_ns();
-    uint32_t spins = 0;
-    while (ld_acquire_gpu(sem) < target) {
-      if (((++spins) & 0x3fu) == 0) {
-        if (*abort_p) { got = false; break; }
-        if (global_timer_ns() - since > kWaitLimitNs) { *abort_p = 1; got = false; break; }
-      }
-      __nanosleep(64);
-    }
-  }
-  return __all_sync(0xffffffffu, got);
-}
-
-}  // namespace
-
-template <int DP, int DH, int BQ, int NSQ, int NSO>
-struct ScoredBwdCfg {
-  static constexpr int kPanels = DP / 64;
-  static constexpr int kHalves = DP / DH;
-  // Head dim 256: K is the A operand of S^T from tensor memory (64 KB, 128 columns), so that shared memory only holds the
-  // half of its columns that dQ^T needs and there is room for a second Q stage.
-  static constexpr bool kKTmem = (DP == 256);
-  static constexpr int kKSmemBytes = 128 * (kKTmem ? DH : DP) * 2;
-  static constexpr int kVBytes = 128 * DP * 2;
-  static constexpr int kQBytes = BQ * DP * 2;
-  static constexpr int kDSBytes = 128 * BQ * 2;
-  static constexpr int kStatBytes = 2 * BQ * 4;
-  static constexpr int kOffK = 0;
-  static constexpr int kOffV = kKSmemBytes;
-  static constexpr int kOffQ = kOffV + kVBytes;
-  static constexpr int kOffDO = kOffQ + NSQ * kQBytes;
-  static constexpr int kOffDS = kOffDO + NSO * kQBytes;
-  static constexpr int kOffStat = kOffDS + kDSBytes;
-  // dQ^T goes through staging buffers to bulk reductions up to head dim 128, two per reduction warp, as in the plain hop.
-  static constexpr bool kStageDQ = (DP <= 128);
-  static constexpr int kDQGroups = (DP == 64) ? BQ / 8 : 4;      // row groups (of 4 query rows) per bulk reduction
-  static constexpr int kDQBufBytes = kDQGroups * 512;            // one warp: 32 lanes x 16 bytes per row group
-  static constexpr int kDQWarps = 2 * (DP < 128 ? DP : 128) / 32;
-  static constexpr int kOffDQ = (kOffStat + NSQ * kStatBytes + 127) / 128 * 128;
-  static constexpr int kSmemUsed = kOffDQ + (kStageDQ ? kDQWarps * 2 * kDQBufBytes : 0);
-  // Pad to more than half of the SM's shared memory so that two CTAs never share an SM
-  // (each CTA allocates the whole tensor memory).
-  static constexpr int kSmemBytes = kSmemUsed < 120 * 1024 ? 120 * 1024 : kSmemUsed;
-  static constexpr int kThreads = 640;
-  static constexpr int kTmS = 0;
-  static constexpr int kTmDP = BQ;
-  static constexpr int kTmDV = 2 * BQ;
-  static constexpr int kTmDK = 2 * BQ + DH;
-  // dQ^T has columns of its own where tensor memory has room for them (head dim 64), so that the next dP^T need not wait
-  // until it is drained; otherwise it takes over those of dP^T.
-  static constexpr bool kOwnDQ = (DP == 64);
-  static constexpr int kTmDQ = kOwnDQ ? 2 * BQ + 2 * DH : kTmDP;
-  static constexpr int kTmK = 2 * BQ + 2 * DH;
-  static_assert(2 * BQ + 2 * DH + (kOwnDQ ? BQ : 0) + (kKTmem ? DP / 2 : 0) <= 512, "tensor memory over budget");
-  static_assert(kSmemBytes <= 232448 - 1024, "shared memory over budget");
 };
 
 // What a CTA works on.  Worked out once and kept in shared memory: each role takes into registers what it needs.
@@ -205,7 +140,7 @@ __global__ void __launch_bounds__(640, 1)
                       const ScoredBwdParams prm) {
   const BwdParams& p = prm.p;
   const ScoreParams& sc = prm.sc;
-  using Cfg = ScoredBwdCfg<DP, DH, BQ, NSQ, NSO>;
+  using Cfg = BwdCfg<DP, DH, BQ, NSQ, NSO>;
   constexpr bool kBf16 = Pack2<T>::kIsBf16;
   constexpr int kShift = weight_shift<T>();
   constexpr int kPanelK = 128 * 128;  // bytes per panel of a 128-row tile
@@ -888,7 +823,7 @@ __global__ void __launch_bounds__(640, 1)
 template <int DP, int DH, int BQ, int NSQ, int NSO, typename T, int kKind>
 static int launch_scored_bwd(const void* q, const void* k, const void* v, const void* dout, const ScoredBwdParams& prm,
                              int dtype, cudaStream_t stream) {
-  using Cfg = ScoredBwdCfg<DP, DH, BQ, NSQ, NSO>;
+  using Cfg = BwdCfg<DP, DH, BQ, NSQ, NSO>;
   const BwdParams& p = prm.p;
   CUtensorMap tq, tk, tv, tdo;
   int rc;
